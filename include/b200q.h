@@ -49,7 +49,7 @@ enum { B200Q_Q8_0 = 8, B200Q_Q4_K = 12, B200Q_Q5_K = 13, B200Q_Q6_K = 14, B200Q_
  * plus a thread-local message (include/sycl_infer/sycl_infer.h:54-59). */
 enum {
     B200Q_OK = 0,
-    B200Q_EINVAL = 1,      /* bad argument: shape, alignment, null pointer */
+    B200Q_EINVAL = 1,      /* bad argument: shape, alignment, null pointer (in the device status: a bad page id) */
     B200Q_EUNSUPPORTED = 2, /* type or size this library has no kernel for */
     B200Q_ECUDA = 3,        /* a CUDA runtime call failed */
     B200Q_ETIMEOUT = 4      /* a bounded device-side wait ran out (see b200q_device_status) */
@@ -322,6 +322,120 @@ int b200q_device_status(int * status /*host*/, int clear);
  * optionally that value.  Calls (and calls with the argmax option) on one device must not overlap:
  * they share device-side words. */
 int b200q_argmax(void * stream, const float * logits, int n, int32_t * out_idx, float * out_val /*may be NULL*/, int M);
+
+/* ---- attention side of a decoder layer: what stands between the q|k|v call and the o call.  The
+ * reference keeps K and V in a pool of fixed-size blocks (32 tokens) that its sequences and its prefix
+ * cache share (src/engine/engine_kvpool, src/engine/engine_prefix_cache), rotates q and k
+ * (src/backend/gpu/kernels/qk_norm_rope.cpp, src/common/yarn.h) and reads the pool with a decode
+ * attention split over the keys (src/backend/gpu/kernels/attn.cpp).  Same roles here.
+ *
+ * Everything that changes from step to step (lengths, row ranges, page tables) is read from device
+ * memory by the kernels, so a recorded launch sequence serves every step. ---- */
+
+/* element types of a cache (ggml ids where ggml has one) */
+enum { B200Q_KV_F16 = 1, B200Q_KV_BF16 = 30, B200Q_KV_E4M3 = 256 };
+
+/* K and V of one layer: pools of n_pages pages of page_size tokens.  Page p, KV head h, token t, value d:
+ *   pool[p * page_stride + (h * page_size + t) * head_dim + d]
+ * A stored element stands for element * k_scale (v_scale).  page_stride (elements) lets several
+ * layers, or K and V, share one allocation. */
+typedef struct b200q_kv_cache {
+    void * k, * v;       /* 16-byte aligned */
+    uint32_t type;       /* B200Q_KV_* */
+    int32_t n_pages;
+    int32_t page_size;   /* 16, 32, 64 or 128 tokens */
+    int32_t n_kv;        /* KV heads */
+    int32_t head_dim;    /* 64 or 128 */
+    int64_t page_stride; /* >= n_kv * page_size * head_dim, a multiple of 16 bytes */
+    float k_scale, v_scale; /* finite, > 0 */
+} b200q_kv_cache;
+
+/* The rows of one step: sequence s owns rows q_start[s] .. q_start[s+1]-1 of every activation buffer, its
+ * newest tokens in order, and kv_len[s] tokens of cache, those new ones included.  Row i of the sequence's
+ * n rows has position kv_len[s] - n + i; a row whose position would be negative has none (it is neither
+ * appended nor rotated, and attention gives zeros for it).  Key j of sequence s lies in page
+ * page_table[s * table_stride + j / page_size].  Rows from q_start[n_seq] on are left as they were.
+ * kv_len beyond table_stride * page_size counts as that.  A table entry outside [0, n_pages) that
+ * a visible key (an appended token) needs: the key is left out (the token not stored), and
+ * b200q_device_status reports B200Q_EINVAL. */
+typedef struct b200q_kv_batch {
+    const int32_t * page_table; /* device */
+    const int32_t * q_start;    /* device, n_seq + 1 entries, non-decreasing, first >= 0, last <= n_tok */
+    const int32_t * kv_len;     /* device, n_seq entries */
+    int32_t table_stride;       /* entries from one sequence's table to the next one's */
+    int32_t n_seq;
+    int32_t n_tok;              /* rows of the activation buffers */
+    int32_t max_q;              /* no sequence has more rows than this (further rows are left as they were) */
+} b200q_kv_batch;
+
+/* Rotary frequencies.  Pair i of a head's n_rot first values turns by theta_i a position,
+ *   theta_i = base^(-2i/n_rot) / freq_factors[i] * freq_scale                  (linear scaling), or with
+ *   ext_factor > 0 the YaRN mix of the scaled and the unscaled frequency: with dim(b) = n_rot *
+ *   ln(n_ctx_orig / (2 pi b)) / (2 ln base), lo = max(0, floor(dim(beta_fast))), hi = min(n_rot - 1,
+ *   ceil(dim(beta_slow))), keep_i = ext_factor * (1 - clamp((i - lo) / max(0.001, hi - lo), 0, 1)):
+ *   theta_i = base^(-2i/n_rot) / freq_factors[i] * (freq_scale * (1 - keep_i) + keep_i),
+ * and the rotated values are multiplied by attn_factor, with YaRN by attn_factor * (1 + 0.1 ln(1/freq_scale))
+ * (Peng et al., "YaRN: Efficient Context Window Extension of Large Language Models", 2023; the reference's
+ * src/common/yarn.h). */
+typedef struct b200q_rope {
+    int32_t n_rot;             /* rotated values of a head, even */
+    int32_t interleaved;       /* 0: pair i is values (i, i + n_rot/2); 1: values (2i, 2i + 1) */
+    float base;                /* > 1 */
+    float freq_scale;          /* 1 / context extension, in (0, 1] */
+    float ext_factor;          /* 0: linear scaling only; YaRN: 1 */
+    float attn_factor;
+    float beta_fast, beta_slow; /* YaRN: 32, 1 */
+    int32_t n_ctx_orig;        /* YaRN: trained context */
+    const float * freq_factors; /* device, n_rot/2 values, or NULL */
+} b200q_rope;
+
+/* Fills the table that b200q_rope_append reads: n_rot/2 frequencies in turns a position, then the factor,
+ * n_rot/2 + 1 doubles.  Once per model. */
+int b200q_rope_table(void * stream, const b200q_rope * rope /*host*/, double * table);
+
+/* Rotates q into q_out (q_out may be q), rotates k and stores it with v as the newest tokens of the
+ * cache.  q, k, v: fp32 rows of n_head * head_dim, n_kv * head_dim values, as the q|k|v call leaves them
+ * (views of one buffer included).  table NULL: no rotation.  q NULL: only the append; k and v NULL (both): only
+ * the rotation of q.  Angles are formed in 64 bits, so positions up to 2^31 keep fp32 accuracy.  Values
+ * beyond the range of an F16 or E4M3 cache are stored as its largest finite value; NaN stays NaN. */
+int b200q_rope_append(void * stream, const double * table, const b200q_rope * rope /*host*/, const float * q,
+                      int q_stride, int n_head, const float * k, int k_stride, const float * v, int v_stride,
+                      float * q_out, int q_out_stride, const b200q_kv_cache * cache /*host*/,
+                      const b200q_kv_batch * batch /*host*/);
+
+/* Attention of the step's rows over the cache: for head h of a row at position p
+ *   out = sum_j w_j v_j,  w = softmax over the visible j of scale * q . k_j,
+ * key j of KV head h / (n_head / n_kv) visible when j <= p and (window == 0 or j > p - window or
+ * j < n_sink).  Rows without a visible key give zeros.  q, out: fp32, one row a token (views included),
+ * out must not overlap q.  K and V are used at full precision; q and the weights are split into two 16-bit
+ * parts for the tensor cores (relative error below 2^-17), sums are fp32.  A NaN or an infinity among the
+ * keys or values that a row sees reaches that row, and may reach other rows of the same sequence in
+ * the same call; keys that no row of the sequence sees are never used.
+ * scratch: b200q_attn_scratch_bytes bytes, 16-byte aligned, zeroed once when it is allocated (the library leaves
+ * its counters zero).  Calls that may overlap on the GPU must not share it. */
+typedef struct b200q_attn_opts {
+    float scale;     /* 0: 1 / sqrt(head_dim) */
+    int32_t window;  /* 0: no window */
+    int32_t n_sink;  /* first tokens that stay visible behind the window */
+} b200q_attn_opts;
+size_t b200q_attn_scratch_bytes(int n_head, int n_kv, int head_dim, int n_seq, int n_tok, int max_q);
+int b200q_attn(void * stream, const float * q, int q_stride, int n_head, const b200q_kv_cache * cache /*host*/,
+               const b200q_kv_batch * batch /*host*/, const b200q_attn_opts * opts /*host, may be NULL*/,
+               float * out, int out_stride, void * scratch, size_t scratch_bytes);
+
+/* Copies page src[i] to page dst[i] of every layer, K and V, for i < n, in one launch per 64 layers: the last
+ * page of a forked sequence, the moves that compact a pool.  The layers' caches differ in k and v only.
+ * dst entries must be distinct and none may also be a src entry of another pair (the copies run at the same
+ * time).  A pair with an entry outside [0, n_pages) is left out and b200q_device_status reports
+ * B200Q_EINVAL. */
+int b200q_kv_copy_pages(void * stream, const b200q_kv_cache * layers /*host*/, int n_layers, const int32_t * src,
+                        const int32_t * dst, int n);
+
+/* out[s * out_stride + i] = map[table[s * table_stride + i]] for i < width, s < n_seq: page tables after
+ * the moves of a compaction (map: n_pages entries, a page's new number).  Entries outside [0, n_pages) stay as
+ * they are.  out may be table (with the same stride). */
+int b200q_kv_remap(void * stream, const int32_t * table, int table_stride, int n_seq, int width, const int32_t * map,
+                   int n_pages, int32_t * out, int out_stride);
 
 /* ---- GGUF files -> one device blob (the loader side of the path: src/model/gguf.{h,cpp} and the
  * whole-file device blob of src/backend/weight_store.h:28-62 in the reference).  The raw block stream

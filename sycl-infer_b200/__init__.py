@@ -9,3 +9,4 @@ through ``__graft_entry__.load_package()`` under the module name ``sycl_infer_b2
 from . import synth  # noqa: F401
 from .capi import Lib, B200QError, load_lib  # noqa: F401
 from .backend import cuda_backend, make_cuda_backend  # noqa: F401
+from .attention import KvPool, alloc_attn_scratch, attn_call, kv_batch, kv_cache, rope_t  # noqa: F401

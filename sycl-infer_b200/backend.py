@@ -16,7 +16,8 @@ from typing import Optional
 
 import torch
 
-from .capi import MAX_SEGS, Seg, load_lib
+from .attention import _int32
+from .capi import MAX_SEGS, AttnOpts, KvCache, Seg, load_lib
 
 
 def _ptr(t):
@@ -51,6 +52,15 @@ class gemv_seg:
         return Seg(_ptr(self.w), self.type, self.K, self.n_rows, _ptr(self.x), self.x_stride, _ptr(self.act_up),
                    _ptr(self.out), self.out_stride or self.n_rows, _ptr(self.residual), self.alpha, _ptr(self.x8),
                    _ptr(self.xmeta), _ptr(self.xsumq))
+
+
+def _rows(t, what, device, width=None):
+    """A 2-D fp32 activation view on `device`, one row a token, unit stride within a row: (pointer, row stride)."""
+    if t.dtype != torch.float32 or t.dim() != 2 or t.device != device or (t.numel() and t.stride(1) != 1):
+        raise ValueError(f"{what}: a 2-D float32 tensor on {device} with unit stride within a row is expected")
+    if width is not None and t.shape[1] != width:
+        raise ValueError(f"{what}: rows of {width} values are expected (got {t.shape[1]})")
+    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else t.shape[1])
 
 
 def _pack(segs):
@@ -199,6 +209,103 @@ class cuda_backend:
         allocate the activation scratch themselves (K <= 32768; calls must not overlap)."""
         arr, n = _pack(segs)
         self.lib.check(self.lib.quant_gemv_static(self._s(), arr, n))
+
+    # ---- attention side: rotary positions + append, attention over the paged cache, page copies ----
+    def _here(self, *tensors):
+        for t in tensors:
+            if t.device != self.device:
+                raise ValueError(f"a tensor on {t.device} was given to the backend of {self.device}")
+
+    def rope_table(self, rope):
+        """Fills rope.table (n_rot / 2 frequencies in turns a position and the factor, 64 bits); once per model."""
+        if rope.table is None:
+            rope.table = torch.empty(max(0, rope.c.n_rot) // 2 + 1, dtype=torch.float64, device=self.device)
+        self._here(rope.table, *([rope.freq_factors] if rope.freq_factors is not None else []))
+        with torch.cuda.device(self.device):
+            self.lib.check(self.lib.rope_table(self._s(), rope.ref, rope.table.data_ptr()))
+        return rope.table
+
+    def rope_append(self, rope, q, k, v, q_out, cache, batch):
+        """Rotates q into q_out (may be q itself) and appends the rotated k, and v, to the cache: the newest
+        tokens of the batch's sequences.  q, k, v: fp32 rows, views of the q|k|v buffer included; rope None:
+        no rotation; q and q_out None: the append alone; k and v None: the rotation of q alone."""
+        if rope is not None and rope.table is None:
+            raise ValueError("rope_append: rope_table() has not been called on this rope_t")
+        self._here(cache, batch, *([rope.table] if rope is not None else []))
+        qp = qs = op = os_ = kp = ks = vp = vs = n_head = 0
+        if (q is None) != (q_out is None) or (k is None) != (v is None):
+            raise ValueError("rope_append: q goes with q_out, k with v")
+        for t in (q, k, v, q_out):
+            if t is not None and t.shape[0] != batch.n_tok:
+                raise ValueError(f"rope_append: {batch.n_tok} rows are expected (got {t.shape[0]})")
+        if q is not None:
+            qp, qs = _rows(q, "rope_append: q", self.device)
+            op, os_ = _rows(q_out, "rope_append: q_out", self.device, q.shape[1])
+            n_head, odd = divmod(q.shape[1], cache.head_dim)
+            if odd:
+                raise ValueError("rope_append: the rows of q are not a multiple of head_dim")
+        if k is not None:
+            kp, ks = _rows(k, "rope_append: k", self.device, cache.n_kv * cache.head_dim)
+            vp, vs = _rows(v, "rope_append: v", self.device, cache.n_kv * cache.head_dim)
+        call = (self._s(), rope.table.data_ptr() if rope is not None else None, rope.ref if rope is not None else None, qp or None,
+                qs, n_head, kp or None, ks, vp or None, vs, op or None, os_, cache.ref, batch.ref)
+        self._on_device(self.lib.rope_append, call)
+
+    def attn(self, q, out, cache, batch, scratch, scale=None, window=0, n_sink=0):
+        """Attention of the batch's rows over the cache (b200q_attn): causal, with `window` the newest `window` keys
+        and the first n_sink ones only.  scratch: attention.alloc_attn_scratch."""
+        self._here(cache, batch, scratch)
+        for t in (q, out):
+            if t.shape[0] != batch.n_tok:
+                raise ValueError(f"attn: {batch.n_tok} rows are expected (got {t.shape[0]})")
+        qp, qs = _rows(q, "attn: q", self.device)
+        op, os_ = _rows(out, "attn: out", self.device, q.shape[1])
+        n_head, odd = divmod(q.shape[1], cache.head_dim)
+        if odd:
+            raise ValueError("attn: the rows of q are not a multiple of head_dim")
+        if batch.n_tok == 0:
+            return
+        if not scratch.is_contiguous():
+            raise ValueError("attn: the scratch must be contiguous")
+        opts = AttnOpts(0.0 if scale is None else float(scale), int(window), int(n_sink))
+        if scale is not None and not scale > 0:
+            raise ValueError("attn: scale must be above 0 (None: 1 / sqrt(head_dim))")
+        call = (self._s(), qp, qs, n_head, cache.ref, batch.ref, C.byref(opts), op, os_, scratch.data_ptr(),
+                scratch.numel() * scratch.element_size())
+        self._on_device(self.lib.attn, call)
+
+    def kv_copy_pages(self, caches, src, dst):
+        """Page src[i] -> page dst[i] in every cache of the list (the layers of a model): int32 device
+        tensors.  dst entries are distinct and none is a src."""
+        caches = list(caches)
+        _int32(src, "kv_copy_pages: src", 1)
+        _int32(dst, "kv_copy_pages: dst", 1)
+        if src.numel() != dst.numel() or not caches:
+            raise ValueError("kv_copy_pages: as many dst as src, and at least one cache")
+        self._here(src, dst, *caches)
+        arr = (KvCache * len(caches))(*[c.c for c in caches])
+        self._on_device(self.lib.kv_copy_pages, (self._s(), arr, len(caches), src.data_ptr() or None, dst.data_ptr() or None, src.numel()))
+
+    def kv_remap(self, table, page_map, out=None):
+        """out[s][i] = page_map[table[s][i]] (in place without out); entries outside the map stay."""
+        out = table if out is None else out
+        for t, n, d in ((table, "table", 2), (out, "out", 2), (page_map, "page_map", 1)):
+            _int32(t, f"kv_remap: {n}", d)
+        if table.shape != out.shape:
+            raise ValueError("kv_remap: out has the table's shape")
+        self._here(table, page_map, out)
+        if table.numel() == 0:
+            return out
+        stride = lambda t: t.stride(0) if t.shape[0] > 1 else t.shape[1]  # noqa: E731
+        self._on_device(self.lib.kv_remap, (self._s(), table.data_ptr(), stride(table), table.shape[0], table.shape[1],
+                                            page_map.data_ptr(), page_map.numel(), out.data_ptr(), stride(out)))
+        return out
+
+    def _on_device(self, fn, args):
+        if torch.cuda.current_device() == self.device.index:
+            return self.lib.check(fn(*args))
+        with torch.cuda.device(self.device):  # launches go to the current device's context
+            self.lib.check(fn(*args))
 
     # parity instrument (no reference operator: the reference never exposes these sums)
     def i8_block_dots(self, w, type, K, n_rows, x8, TB, t, wd):

@@ -9,7 +9,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libb200q.so")
 STAMP = os.path.join(HERE, "build", "libb200q.stamp")
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-shared",
-              "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall"]
+              "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall", "--threads", "0"]
 
 
 def _nvcc():

@@ -76,6 +76,34 @@ class GgufTensor(C.Structure):
                 ("shard", C.c_int32), ("host_data", _vp)]
 
 
+KV_TYPES = {"F16": 1, "BF16": 30, "E4M3": 256}
+
+
+class KvCache(C.Structure):
+    """struct b200q_kv_cache."""
+    _fields_ = [("k", _vp), ("v", _vp), ("type", C.c_uint32), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+                ("n_kv", C.c_int32), ("head_dim", C.c_int32), ("page_stride", C.c_int64), ("k_scale", C.c_float),
+                ("v_scale", C.c_float)]
+
+
+class KvBatch(C.Structure):
+    """struct b200q_kv_batch."""
+    _fields_ = [("page_table", _vp), ("q_start", _vp), ("kv_len", _vp), ("table_stride", C.c_int32), ("n_seq", C.c_int32),
+                ("n_tok", C.c_int32), ("max_q", C.c_int32)]
+
+
+class Rope(C.Structure):
+    """struct b200q_rope."""
+    _fields_ = [("n_rot", C.c_int32), ("interleaved", C.c_int32), ("base", C.c_float), ("freq_scale", C.c_float),
+                ("ext_factor", C.c_float), ("attn_factor", C.c_float), ("beta_fast", C.c_float), ("beta_slow", C.c_float),
+                ("n_ctx_orig", C.c_int32), ("freq_factors", _vp)]
+
+
+class AttnOpts(C.Structure):
+    """struct b200q_attn_opts."""
+    _fields_ = [("scale", C.c_float), ("window", C.c_int32), ("n_sink", C.c_int32)]
+
+
 _SIGS = {
     "b200q_last_error": (C.c_char_p, []),
     "b200q_version": (C.c_int, []),
@@ -104,6 +132,12 @@ _SIGS = {
     "b200q_i8_block_dots": (C.c_int, [_vp, _vp, C.c_uint32, C.c_int, C.c_int, _vp, C.c_int, C.c_int, _vp]),
     "b200q_device_status": (C.c_int, [C.POINTER(C.c_int), C.c_int]),
     "b200q_argmax": (C.c_int, [_vp, _vp, C.c_int, _vp, _vp, C.c_int]),
+    "b200q_rope_table": (C.c_int, [_vp, _vp, _vp]),
+    "b200q_rope_append": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, C.c_int, _vp, C.c_int, _vp, C.c_int, _vp, C.c_int, _vp, _vp]),
+    "b200q_attn_scratch_bytes": (C.c_size_t, [C.c_int] * 6),
+    "b200q_attn": (C.c_int, [_vp, _vp, C.c_int, C.c_int, _vp, _vp, _vp, _vp, C.c_int, _vp, C.c_size_t]),
+    "b200q_kv_copy_pages": (C.c_int, [_vp, C.POINTER(KvCache), C.c_int, _vp, _vp, C.c_int]),
+    "b200q_kv_remap": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, _vp, C.c_int, _vp, C.c_int]),
     "b200q_gguf_open": (C.c_int, [C.c_char_p, C.POINTER(_vp)]),
     "b200q_gguf_close": (None, [_vp]),
     "b200q_gguf_n_tensors": (C.c_int, [_vp]),

@@ -1,0 +1,88 @@
+// What the attention kernels share: arguments, the keys that a sequence's rows see, 16-bit splitting.
+#pragma once
+#include <type_traits>
+
+#include "kv.cuh"
+#include "launch.h"
+
+namespace b200q {
+
+struct AttnDev {
+    const float * q;
+    float * out;
+    int32_t q_stride, out_stride, n_head, group; // group: query heads of a KV head
+    KvDev kv;
+    BatchDev b;
+    float scale_log2; // softmax scale x log2(e) x k_scale
+    float v_scale;
+    int32_t window, n_sink;
+    float * parts;       // scratch: what CTAs leave of units that they share
+    uint32_t * counters; // scratch: arrivals a unit, zero between calls
+    int32_t row_blocks;  // row blocks of a (sequence, KV head) at most
+    int32_t min_tiles;   // tiles that a CTA gets at least
+};
+
+cudaError_t launch_attn_decode(cudaStream_t s, AttnDev a);
+size_t attn_decode_units(int n_head, int n_kv, int n_seq, int max_q);
+size_t attn_decode_part_bytes(int n_head, int n_kv, int head_dim, int max_q);
+
+#ifdef __CUDACC__
+
+// Tiles of `kt` keys that some row of a sequence sees: those of the first n_sink keys, then those from the oldest
+// key in any row's window to the newest.  At least one, so that rows that see nothing are still written.
+struct KeyTiles {
+    int oldest;     // oldest key in any row's window
+    int sink_tiles; // tiles of the list that belong to the sinks alone
+    int t_lo;       // tile of `oldest`
+    int count;
+};
+__device__ __forceinline__ KeyTiles key_tiles(const SeqRows & r, int kt, int window, int n_sink) {
+    KeyTiles k;
+    const int pos_first = r.n - r.n_row;
+    k.oldest = window ? max(0, pos_first - window + 1) : 0;
+    k.oldest = min(k.oldest, r.n);
+    k.t_lo = k.oldest / kt;
+    k.sink_tiles = min((min(n_sink, r.n) + kt - 1) / kt, k.t_lo);
+    k.count = max(1, k.sink_tiles + (r.n + kt - 1) / kt - k.t_lo);
+    return k;
+}
+__device__ __forceinline__ int key_tile(const KeyTiles & k, int i) { return i < k.sink_tiles ? i : i - k.sink_tiles + k.t_lo; }
+
+__device__ __forceinline__ float exp2_fast(float x) { // 2 ulp, 0 for -inf
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The power of two that brings `top` into [2^14, 2^15), kept within fp32's exponents; 0 for zero, infinity and NaN.
+__device__ __forceinline__ int pow2_to_top(float top) {
+    const int e = (int)((__float_as_uint(top) >> 23) & 255u);
+    return e == 0 || e == 255 ? 0 : min(14 - (e - 127), 126);
+}
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); } // -126..127
+
+// (x, y) = hi + lo in two pairs of 16-bit numbers
+template <int T> __device__ __forceinline__ void split2(float x, float y, uint32_t & hi, uint32_t & lo) {
+    if constexpr (T == kBF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        hi = *reinterpret_cast<const uint32_t *>(&h);
+        const __nv_bfloat162 r = __floats2bfloat162_rn(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xFFFF0000u));
+        lo = *reinterpret_cast<const uint32_t *>(&r);
+    } else {
+        const __half2 h = __floats2half2_rn(x, y);
+        hi = *reinterpret_cast<const uint32_t *>(&h);
+        const float2 f = __half22float2(h);
+        const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
+        lo = *reinterpret_cast<const uint32_t *>(&r);
+    }
+}
+
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t v) { // the low 16 bits; exact
+    uint32_t r;
+    asm("{.reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t;}" : "=r"(r) : "r"(v));
+    return r;
+}
+
+#endif
+
+} // namespace b200q

@@ -709,8 +709,18 @@ int b200q_device_status(int * status, int clear) {
     int probe = 0;
     B200Q_CUDA_OK(read_probe_status(&probe, clear != 0));
     *status = *status ? *status : probe;
+    int page = 0, word = 0;
+    B200Q_CUDA_OK(read_append_status(&word, clear != 0));
+    page = page ? page : word;
+    B200Q_CUDA_OK(read_attn_status(&word, clear != 0));
+    page = page ? page : word;
+    B200Q_CUDA_OK(read_pages_status(&word, clear != 0));
+    page = page ? page : word;
     if (*status != 0) {
         set_error("a bounded device-side wait ran out (status %d)", *status);
+    } else if (page != 0) {
+        set_error("a page table or a list of pages named a page outside the pool (status %d)", page);
+        *status = page;
     }
     return B200Q_OK;
 }

@@ -4,14 +4,16 @@ A layer is four *calls* in the reference engine's sense (seg_plan::call_t,
 src/engine/engine_types.h:46-61 of the reference): q|k|v (three segments sharing the
 quantized hidden state), o, gate|up (two segments writing the halves of one 2*n_ff
 buffer, src/engine/graph.cpp:342-343) and down (activation silu(gate)*up, residual add
-in place, graph.cpp:355-357).  Attention itself is outside this path: the o call reads
-a fixed device vector.  With world > 1 every weight is sharded by output rows
+in place, graph.cpp:355-357).  Without a cache the o call reads a fixed device vector (the
+GEMV path alone); `attach_attention` puts rotary positions, the append to a paged cache and
+attention between q|k|v and o.  With world > 1 every weight is sharded by output rows
 (sharding.shard_rows) and each call's outputs are all-gathered before the next call
 consumes them.
 """
 import torch
 
 from . import synth
+from .attention import attn_call
 from .backend import alloc_act, gemv_seg
 from .sharding import gather_rows, shard_rows
 
@@ -63,6 +65,19 @@ class DenseLayer:
         # 58.3): two large kernel images taking turns on the SMs cost more than the boundaries save.
         self.chain = False
         self._staging = {}
+        self.attention = None
+
+    def attach_attention(self, cache, batch, scratch, rope=None, scale=None, window=0, n_sink=0):
+        """From here on forward() rotates q and k, appends k and v to `cache` and attends (attention.attn_call);
+        the batch has TB rows.  One GPU: the q|k|v rows of a sharded layer do not follow the heads."""
+        if self.world > 1:
+            raise ValueError("attach_attention: a row-sharded layer has no whole heads")
+        if batch.n_tok != self.TB:
+            raise ValueError(f"attach_attention: the layer runs {self.TB} rows, the batch has {batch.n_tok}")
+        q, k, v = self.qkv.split([self.q_dim, self.kv_dim, self.kv_dim], 1)
+        call = attn_call(q, k, v, self.attn, cache, batch, scratch, rope, scale, window, n_sink)
+        call.validate("attach_attention")
+        self.attention = call
 
     def weight_bytes(self):
         return sum(int(w.numel()) for w in self.w.values())
@@ -97,10 +112,14 @@ class DenseLayer:
         calls = calls or self.calls(x, out)
         if self.fused_h and self.chain:
             self.be.quant_gemv_ex(calls[0][0], 1)
+            if self.attention is not None:
+                self.attention.run(self.be)
             self.be.quant_gemv_chain([(calls[1][0], False, None), (calls[2][0], False, self.act_f),
                                       (calls[3][0], True, None)])
             return out
         for i, (segs, gathers) in enumerate(calls):
+            if i == 1 and self.attention is not None:
+                self.attention.run(self.be)
             if self.fused_h:
                 # one launch per call: q|k|v and o quantize in the GEMV's prologue, gate|up emits down's
                 # quantized activation
@@ -129,8 +148,9 @@ class DenseLayer:
     def launches_per_step(self):
         # single token on one GPU: q|k|v, o and gate|up quantize in the GEMV's prologue and gate|up
         # also emits down's quantized activation: one launch per call; otherwise a quantizer + GEMV per call
+        attn = 2 if self.attention is not None else 0  # rotary positions + append, attention
         if self.arena is not None:  # GEMV with peer stores; down keeps its silu(gate)*up quantizer launch
             return 5 if self.TB == 1 else 12
         if self.fused_h:
-            return 2 if self.chain else 4
-        return 5 if self.TB == 1 else 8
+            return attn + (2 if self.chain else 4)
+        return attn + (5 if self.TB == 1 else 8)

@@ -7,7 +7,8 @@ src/engine/graph.cpp:145-429).  `SegPlan` mirrors that structure (begin_call / a
 finalize, same meaning) and adds what this library can do with it: `finalize()` lowers the calls to
 launches, pairing a gate|up call with the down call that consumes silu(gate)*up (the former emits
 the latter's quantized activation, the latter runs without a quantizer), folding a call's RMSNorm
-into its quantizer and hanging the argmax on the head call; `record()` captures the launches of a
+into its quantizer and hanging the argmax on the head call (routed-MoE and attention calls bring launch
+sequences of their own); `record()` captures the launches of a
 whole token into ONE CUDA graph and `replay()` runs it.
 
 `PlanBuckets` mirrors the engine's decode buckets (src/engine/engine.h:770-782, src/engine/graph.cpp:
@@ -33,6 +34,8 @@ class Call:
     argmax: tuple = None      # (idx, val or None): argmax of the outputs (the head call)
     # a routed-MoE call has no segments: it dispatches the MoE launch sequence (call_t::moe_routed)
     moe: tuple = None         # (moe_t, MoeScratch, out): out[t] += sum_j w[t,j] * expert(x[t])
+    # an attention call has none either: rotary positions + append, then attention over the paged cache
+    attn: object = None       # attention.attn_call
     # set by finalize()
     prequantized: bool = False
     next_act: tuple = None
@@ -75,6 +78,13 @@ class SegPlan:
         self.calls.append(Call(tb=tb, x=x, moe=(M, scratch, out)))
         self.lowered = None
 
+    def begin_attn_call(self, call):
+        """The attention of a layer in the call sequence, between its q|k|v call and its o call: rotary positions with
+        the append to the cache, then attention (attention.attn_call).  The step's lengths and tables are device
+        data, so the recorded graph serves every step."""
+        self.calls.append(Call(tb=call.batch.n_tok, attn=call))
+        self.lowered = None
+
     # ---- validation + lowering ------------------------------------------------------------------
     def validate(self):
         """Structural self-check (seg_plan::validate): raises ValueError naming the first violation."""
@@ -82,6 +92,11 @@ class SegPlan:
             if c.moe is not None:
                 if c.segs or c.x is None or c.norm or c.argmax:
                     raise ValueError(f"call {ci}: a MoE call has an activation and nothing else")
+                continue
+            if c.attn is not None:
+                if c.segs or c.x is not None or c.norm or c.argmax:
+                    raise ValueError(f"call {ci}: an attention call has its own rows and nothing else")
+                c.attn.validate(f"call {ci}")
                 continue
             if not 1 <= len(c.segs) <= MAX_SEGS:
                 raise ValueError(f"call {ci}: {len(c.segs)} segments (1..{MAX_SEGS})")
@@ -123,6 +138,8 @@ class SegPlan:
         for c in self.calls:
             if c.moe is not None:
                 n += 7  # token quantizer, router logits, softmax/top-k + CSR, gate|up, quantizer of h, down, reduce
+            elif c.attn is not None:
+                n += 2  # rotary positions + append, attention
             else:
                 n += 1 if c.prequantized or (c.tb == 1 and c.up is None) else 2
         return n
@@ -135,6 +152,9 @@ class SegPlan:
             if c.moe is not None:
                 M, scratch, out = c.moe
                 moe_call(be, M, scratch, c.x, c.tb, out)
+                continue
+            if c.attn is not None:
+                c.attn.run(be)
                 continue
             segs = []
             # the segments carry the call's activation, as the C ABI wants it; a 2-D activation may be a
