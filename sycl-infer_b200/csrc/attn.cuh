@@ -57,23 +57,26 @@ __device__ __forceinline__ float exp2_fast(float x) { // 2 ulp, 0 for -inf
 // The power of two that brings `top` into [2^14, 2^15), kept within fp32's exponents; 0 for zero, infinity and NaN.
 __device__ __forceinline__ int pow2_to_top(float top) {
     const int e = (int)((__float_as_uint(top) >> 23) & 255u);
-    return e == 0 || e == 255 ? 0 : min(14 - (e - 127), 126);
+    return e == 0 || e == 255 ? 0 : min(14 - (e - 127), 100);
 }
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); } // -126..127
 
-// (x, y) = hi + lo in two pairs of 16-bit numbers
-template <int T> __device__ __forceinline__ void split2(float x, float y, uint32_t & hi, uint32_t & lo) {
-    if constexpr (T == kBF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-        hi = *reinterpret_cast<const uint32_t *>(&h);
-        const __nv_bfloat162 r = __floats2bfloat162_rn(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xFFFF0000u));
-        lo = *reinterpret_cast<const uint32_t *>(&r);
-    } else {
-        const __half2 h = __floats2half2_rn(x, y);
-        hi = *reinterpret_cast<const uint32_t *>(&h);
-        const float2 f = __half22float2(h);
-        const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
-        lo = *reinterpret_cast<const uint32_t *>(&r);
+// (x, y) as a sum of N pairs of 16-bit numbers, the largest first
+template <int T, int N> __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&part)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if constexpr (T == kBF16) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+            part[i] = *reinterpret_cast<const uint32_t *>(&h);
+            x -= __uint_as_float(part[i] << 16);
+            y -= __uint_as_float(part[i] & 0xFFFF0000u);
+        } else {
+            const __half2 h = __floats2half2_rn(x, y);
+            part[i] = *reinterpret_cast<const uint32_t *>(&h);
+            const float2 f = __half22float2(h);
+            x -= f.x;
+            y -= f.y;
+        }
     }
 }
 

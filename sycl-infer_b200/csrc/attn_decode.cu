@@ -9,19 +9,22 @@
 //   KV head, so that K and V are read once for all of them.  The units' key tiles in order form one list,
 //   and the CTAs take equal contiguous shares of it, whatever the lengths: a long sequence is split
 //   over many CTAs, short ones are several to a CTA.  Lengths are read on the device.
-// * Streams.  Each warp takes every fourth tile of the CTA's share of a unit and owns a ring of three 8 KB
-//   stages that it fills by itself with 16-byte asynchronous copies: no block barrier inside the stream, and the ring runs
-//   on over the units' borders, so that the next unit's keys travel while the last one is joined.
-// * Products on mma.sync m16n8k16: with at most 16 query rows the tensor work is a few per cent of the time that the
-//   tile's bytes take, and a 128-row tcgen05 tile would be empty.  fp32 accuracy at 16-bit operands: q and p are
-//   split into two 16-bit parts, x = hi + lo.  Up to eight rows, the sixteen rows of the one product are the
-//   eight hi and the eight lo rows, and the two halves of the accumulators are added; more rows take two products.
-//   bf16 caches: 16 bits of q and p (off by at most 2^-18 of the value); fp16 and e4m3 caches (e4m3 becomes fp16 exactly):
-//   22 bits, with q scaled per row by a power of two to the top of fp16's range and p by 2^14, so that small parts do
-//   not fall below fp16's smallest step.
-// * Join.  The four warps' (m, l, o) are joined in shared memory in a fixed order; where a unit spans CTAs, each
-//   leaves its part in the scratch and the CTA that finishes last joins the parts in order, so results do not depend
-//   on who that is.
+// * Streams.  Each warp owns a ring of three 8 KB stages that it fills by itself with 16-byte asynchronous copies: no
+//   block barrier inside the stream, and the ring runs on over the units' borders, so that the next unit's keys
+//   travel while the last one is finished.
+// * Teams.  With many units every warp is a worker with a share of its own (TEAM 1); with few, the four warps of a CTA
+//   take every fourth tile of a common share and join in shared memory (TEAM 4), so that a unit is left in
+//   fewer parts.
+// * Products on mma.sync m16n8k16: with at most 16 query rows the tensor work hides behind the bytes, and a 128-row
+//   tcgen05 tile would be empty.  fp32 accuracy at 16-bit operands: q and p are split into 16-bit parts, two for
+//   fp16 and e4m3 caches (e4m3 becomes fp16 exactly; 22 bits, with q scaled per row by a power of two to the top of
+//   fp16's range and p by 2^14, so that small parts do not fall below fp16's smallest step), three for bf16 (24 bits).
+//   Up to eight rows, the sixteen rows of one product are the eight first and the eight second parts.  The tensor
+//   cores' fp32 sums drop bits at every step, always towards zero, so a long chain drifts: each tile's product starts from
+//   zero, smallest parts first, and is added to the running o in a rounded fp32 addition (which the rescaling to the new
+//   maximum needs anyway).
+// * Join.  Where a unit spans workers, each leaves its (m, l, o) in the scratch and the one that finishes last joins the
+//   parts in order, so results do not depend on who that is.
 #include "async.cuh"
 #include "attn.cuh"
 
@@ -64,8 +67,8 @@ __device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&v)[4]) {
 __device__ __forceinline__ void lds128(uint32_t a, uint32_t (&v)[4]) {
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a) : "memory");
 }
-__device__ __forceinline__ void lds64(uint32_t a, uint32_t & x, uint32_t & y) {
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x), "=r"(y) : "r"(a) : "memory");
+__device__ __forceinline__ void lds64(uint32_t a, uint32_t (&v)[2]) {
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a) : "memory");
 }
 // copies 16 bytes, or fills with zeros where `take` is false
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void * src, bool take) {
@@ -84,7 +87,7 @@ template <int T> __device__ __forceinline__ void mma16816(float (&d)[4], const u
     }
 }
 
-// The unit that a CTA works on, and its share of the unit's tiles.
+// The unit that a worker is at, and its share of the unit's tiles.
 struct Segment {
     int s, h, rb;        // sequence, KV head, row block
     int t_begin, t_end;  // tiles of the unit's list
@@ -104,28 +107,36 @@ template <int KT, int ROWS> __device__ __forceinline__ SeqTiles seq_tiles(const 
     return q;
 }
 
-// H8: at most eight rows a unit, hi and lo parts side by side in one product; otherwise sixteen rows, two products.
-template <int T, int D, bool H8> __global__ void __launch_bounds__(kDecThreads, kDecPerSM) attn_decode_kernel(const __grid_constant__ AttnDev a) {
+// Floats of a part in the scratch or in shared memory: o as the warp's threads hold it, then (m, l) of up to 16 rows.
+__host__ __device__ constexpr int part_floats(int dim, bool h8) { return (dim / 8 * (h8 ? 2 : 4) + 1) * 32; }
+
+// H8: at most eight rows a unit, first and second parts side by side in one product; otherwise sixteen rows.
+template <int T, int D, bool H8, int TEAM>
+__global__ void __launch_bounds__(kDecThreads, kDecPerSM) attn_decode_kernel(const __grid_constant__ AttnDev a) {
     constexpr int EB = KvElem<T>::BYTES, ROWB = D * EB, KT = kDecStageBytes / 2 / ROWB;
     constexpr int ROWS = H8 ? 8 : 16, KS = D / 16, NT = D / 8;
+    constexpr int PARTS = T == kBF16 ? 3 : 2;  // 16-bit parts of q and p
+    constexpr int NA = H8 ? PARTS - 1 : PARTS; // A operands: with H8 the first holds two parts
     constexpr int CPR = ROWB / 16;             // 16-byte chunks of a row
     constexpr int RPI = 32 / CPR;              // rows that one copy instruction of the warp covers
+    constexpr int GROUPS = KT / 16;            // groups of 16 keys: contiguous in a page
     constexpr int OV = H8 ? 2 : 4;             // o values of a thread per 8 columns
+    constexpr int RX = H8 ? 1 : 2;             // rows of a thread
     constexpr float kPBias = T == kBF16 ? 0.0f : 14.0f;
-    constexpr int PART = (NT * OV + 1) * 32;   // floats of a part: o, then (m, l) of the up to sixteen rows
+    constexpr int PART = part_floats(D, H8);
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long s_sum[kDecWarps], s_before;
-    __shared__ int s_seq, s_last;
+    __shared__ long long s_sum[kDecWarps], s_before[kDecWarps];
+    __shared__ int s_seq[kDecWarps], s_last;
     __shared__ int2 s_meta[kDecWarps][kDecStages];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * kDecStages * kDecStageBytes;
-    float * join = reinterpret_cast<float *>(smem + kDecWarps * kDecStages * kDecStageBytes); // two parts
+    float * join = reinterpret_cast<float *>(smem + kDecWarps * kDecStages * kDecStageBytes); // TEAM 4: two parts
 
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // ---- the CTA's share [c0, c1) of the list of all units' tiles
-    auto block_sum = [&](long long v, long long & before) { // inclusive over threads; returns the block's sum
+    // ---- the worker's share [c0, c1) of the list of all units' tiles
+    auto block_sum = [&](long long v, long long & before) { // before: sum over the threads below; returns the block's sum
         long long x = v;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -153,41 +164,57 @@ template <int T, int D, bool H8> __global__ void __launch_bounds__(kDecThreads, 
         const SeqTiles q = seq_tiles<KT, ROWS>(a, s);
         return (long long)q.blocks * q.k.count * a.kv.n_kv;
     };
-    long long total = 0, before;
-    for (int s0 = 0; s0 < a.b.n_seq; s0 += kDecThreads) {
+    const long long v_first = seq_total(tid);
+    long long before_first, before;
+    long long total = block_sum(v_first, before_first);
+    const long long sum_first = total;
+    for (int s0 = kDecThreads; s0 < a.b.n_seq; s0 += kDecThreads) {
         total += block_sum(seq_total(s0 + tid), before);
     }
     if (total == 0) {
         return;
     }
-    const long long want = (total + a.min_tiles - 1) / a.min_tiles;
-    const long long nw = want < gridDim.x ? want : gridDim.x;
-    if (blockIdx.x >= nw) {
+    constexpr int WORKERS = kDecWarps / TEAM; // of a CTA
+    const long long want = (total + a.min_tiles - 1) / a.min_tiles, most = (long long)gridDim.x * WORKERS;
+    const long long nw = want < most ? want : most;
+    if ((long long)blockIdx.x * WORKERS >= nw) {
         return;
     }
-    const long long c0 = blockIdx.x * total / nw, c1 = (blockIdx.x + 1) * total / nw;
+    const int worker = blockIdx.x * WORKERS + warp / TEAM;
+    const long long c0 = worker * total / nw, c1 = (worker + 1) * total / nw;
     {
         long long run = 0;
         for (int s0 = 0; s0 < a.b.n_seq; s0 += kDecThreads) {
-            const long long v = seq_total(s0 + tid);
-            const long long all = block_sum(v, before);
-            if (v > 0 && c0 >= run + before && c0 < run + before + v) {
-                s_seq = s0 + tid;
-                s_before = run + before;
+            long long v = v_first, all = sum_first;
+            before = before_first;
+            if (s0 > 0) {
+                v = seq_total(s0 + tid);
+                all = block_sum(v, before);
+            }
+#pragma unroll
+            for (int w = 0; w < WORKERS; w++) {
+                const long long c = (blockIdx.x * WORKERS + w) * total / nw;
+                if (v > 0 && c >= run + before && c < run + before + v) {
+                    s_seq[w] = s0 + tid;
+                    s_before[w] = run + before;
+                }
             }
             run += all;
-            if (run > c0) {
+            if (run > (blockIdx.x * WORKERS + WORKERS - 1) * total / nw) {
                 break;
             }
         }
         __syncthreads();
     }
+    if (worker >= nw) {
+        return; // TEAM 1 only: no block barrier from here on
+    }
     // the first unit
     Segment first;
     {
-        first.s = s_seq;
+        first.s = s_seq[warp / TEAM];
         const SeqTiles q = seq_tiles<KT, ROWS>(a, first.s);
-        long long at = c0 - s_before;
+        const long long at = c0 - s_before[warp / TEAM];
         const int u = (int)(at / q.k.count);
         first.h = u / q.blocks;
         first.rb = u % q.blocks;
@@ -196,7 +223,7 @@ template <int T, int D, bool H8> __global__ void __launch_bounds__(kDecThreads, 
         const long long left = c1 - c0, here = q.k.count - first.t_begin;
         first.t_end = first.t_begin + (int)(left < here ? left : here);
     }
-    // the next unit after `g`, `left` tiles of the share still to come (> 0)
+    // the unit after x, with `left` tiles of the share still to come (> 0)
     auto advance = [&](Segment & x, long long left, SeqTiles & q) {
         if (++x.rb == q.blocks) {
             x.rb = 0;
@@ -212,13 +239,15 @@ template <int T, int D, bool H8> __global__ void __launch_bounds__(kDecThreads, 
         x.t_begin = 0;
         x.t_end = (int)(left < q.k.count ? left : q.k.count);
     };
+    const int w_first = TEAM == 1 ? 0 : warp; // the warp's first tile of a segment
 
-    // ---- the warp's stream: issue() copies the warp's next tile into a stage and says whether there was one
+    // ---- the warp's stream: issue() copies the warp's next tile into the next stage
     Segment ps = first;
     SeqTiles pq = seq_tiles<KT, ROWS>(a, ps.s);
     long long p_left = c1 - c0; // tiles from the start of ps on
-    int p_tile = ps.t_begin + warp;
-    int n_issued = 0;
+    int p_tile = ps.t_begin + w_first;
+    int p_stage = 0;
+    const int copy_row = lane / CPR, copy_chunk = lane % CPR;
     auto issue = [&]() {
         while (p_tile >= ps.t_end) {
             p_left -= ps.t_end - ps.t_begin;
@@ -227,49 +256,61 @@ template <int T, int D, bool H8> __global__ void __launch_bounds__(kDecThreads, 
                 return;
             }
             advance(ps, p_left, pq);
-            p_tile = ps.t_begin + warp;
+            p_tile = ps.t_begin + w_first;
         }
-        const int stage = n_issued % kDecStages;
         const int tile = key_tile(pq.k, p_tile);
         const int key0 = tile * KT;
-        // pages of the tile's groups of 16 keys, one a lane
-        constexpr int GROUPS = KT / 16;
-        int page = -1;
-        bool bad = false;
+        // lane i looks after the tile's group i: where its 16 rows lie, which of them some row sees
+        unsigned long long src = 0;
+        uint32_t seen = 0;
         if (lane < GROUPS) {
             const int k0 = key0 + lane * 16;
-            // a group none of whose keys any row sees needs no page
             if (k0 < pq.r.n && (k0 + 15 >= pq.k.oldest || k0 < a.n_sink)) {
-                page = a.b.page_table[(size_t)ps.s * a.b.table_stride + (k0 >> a.kv.page_shift)];
-                if (page < 0 || page >= a.kv.n_pages) {
-                    page = -1;
-                    bad = true;
+                const int page = a.b.page_table[(size_t)ps.s * a.b.table_stride + (k0 >> a.kv.page_shift)];
+                if (page >= 0 && page < a.kv.n_pages) {
+                    src = (unsigned long long)page * a.kv.page_bytes +
+                          (((unsigned long long)ps.h << a.kv.page_shift) + (k0 & ((1 << a.kv.page_shift) - 1))) * ROWB;
+                    seen = k0 + 16 <= pq.r.n ? 0xFFFFu : 0xFFFFu >> (k0 + 16 - pq.r.n);
+                    if (k0 < pq.k.oldest) {
+                        uint32_t keep = pq.k.oldest - k0 >= 16 ? 0u : 0xFFFFu << (pq.k.oldest - k0);
+                        keep |= a.n_sink - k0 >= 16 ? 0xFFFFu : (a.n_sink > k0 ? 0xFFFFu >> (16 - (a.n_sink - k0)) : 0u);
+                        seen &= keep;
+                    }
+                } else {
+                    atomicExch(&g_attn_status, B200Q_EINVAL);
                 }
             }
         }
-        if (bad) {
-            atomicExch(&g_attn_status, B200Q_EINVAL);
-        }
-        const uint32_t valid = __ballot_sync(~0u, page >= 0);
+        const uint32_t valid = __ballot_sync(~0u, seen != 0), full = __ballot_sync(~0u, seen == 0xFFFFu);
         if (lane == 0) {
-            s_meta[warp][stage] = make_int2(tile, (int)valid);
+            s_meta[warp][p_stage] = make_int2(key0, (int)valid);
         }
-        const uint32_t dk = ring + stage * kDecStageBytes, dv = dk + kDecStageBytes / 2;
-        const int c = lane % CPR, r0 = lane / CPR;
+        const uint32_t dk = ring + p_stage * kDecStageBytes, dv = dk + kDecStageBytes / 2;
 #pragma unroll
-        for (int i = 0; i < KT / RPI; i++) {
-            const int r = i * RPI + r0, key = key0 + r;
-            const int pg = __shfl_sync(~0u, page, (i * RPI) / 16);
-            const bool take = pg >= 0 && key < pq.r.n && (key >= pq.k.oldest || key < a.n_sink);
-            const size_t off = (size_t)max(pg, 0) * a.kv.page_bytes +
-                               (((size_t)ps.h << a.kv.page_shift) + (key & ((1 << a.kv.page_shift) - 1))) * ROWB + c * 16;
-            const uint32_t so = tile_off<T, ROWB>(r, c);
-            cp_async16_or_zero(dk + so, a.kv.k + off, take);
-            cp_async16_or_zero(dv + so, a.kv.v + off, take);
+        for (int gr = 0; gr < GROUPS; gr++) {
+            const unsigned long long off = __shfl_sync(~0u, src, gr) + lane * 16;
+            const uint8_t * fk = a.kv.k + off, * fv = a.kv.v + off;
+            if ((full >> gr) & 1) {
+#pragma unroll
+                for (int i = 0; i < 16 / RPI; i++) {
+                    const uint32_t so = tile_off<T, ROWB>(gr * 16 + i * RPI + copy_row, copy_chunk);
+                    cp_async16(dk + so, fk + i * 512);
+                    cp_async16(dv + so, fv + i * 512);
+                }
+            } else { // rows that nobody sees (their memory may hold anything) become zeros
+                const uint32_t rows = __shfl_sync(~0u, seen, gr);
+#pragma unroll
+                for (int i = 0; i < 16 / RPI; i++) {
+                    const uint32_t so = tile_off<T, ROWB>(gr * 16 + i * RPI + copy_row, copy_chunk);
+                    const bool take = (rows >> (i * RPI + copy_row)) & 1;
+                    cp_async16_or_zero(dk + so, take ? fk + i * 512 : a.kv.k, take);
+                    cp_async16_or_zero(dv + so, take ? fv + i * 512 : a.kv.v, take);
+                }
+            }
         }
         cp_async_commit();
-        n_issued++;
-        p_tile += kDecWarps;
+        p_stage = p_stage + 1 == kDecStages ? 0 : p_stage + 1;
+        p_tile += TEAM;
     };
 #pragma unroll
     for (int i = 0; i < kDecStages - 1; i++) {
@@ -280,29 +321,31 @@ template <int T, int D, bool H8> __global__ void __launch_bounds__(kDecThreads, 
     Segment sg = first;
     SeqTiles sq = seq_tiles<KT, ROWS>(a, sg.s);
     long long left = c1 - c0, at = c0;
-    int done = 0;
+    int stage = 0;
     for (;;) {
         // rows: a thread holds row g, and with sixteen rows row g + 8 too
-        int row_tok[2], row_head[2], pos[2];
-        bool live[2];
+        int row_tok[RX], row_head[RX], pos[RX];
+        bool live[RX];
         const int n_rows = sq.r.n_run * a.group;
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
+        for (int x = 0; x < RX; x++) {
             const int r = sg.rb * ROWS + g + 8 * x;
-            live[x] = (x == 0 || !H8) && r < n_rows;
+            live[x] = r < n_rows;
             const int i = live[x] ? r / a.group : 0;
             row_tok[x] = sq.r.row0 + i;
             row_head[x] = sg.h * a.group + (live[x] ? r - i * a.group : 0);
             pos[x] = live[x] ? sq.r.n - sq.r.n_row + i : -1;
         }
-        // q as fragments: qa[k step][0] (H8: hi rows above lo rows; else the hi parts), [1] the lo parts
-        uint32_t qa[KS][H8 ? 1 : 2][4];
-        float cq[2] = {a.scale_log2, a.scale_log2};
+        // q as A operands.  H8: qa[.][0] has the first parts in rows 0..7 and the second in 8..15, qa[.][1] the third parts
+        // in rows 0..7; otherwise qa[.][y] has part y of the sixteen rows.
+        uint32_t qa[KS][NA][4];
+        float cq[RX];
         {
-            float qv[KS][2][4]; // [k step][row][slots 2t, 2t+1, 2t+8, 2t+9]
+            float qv[KS][RX][4]; // [k step][row][slots 2t, 2t+1, 2t+8, 2t+9]
 #pragma unroll
-            for (int x = 0; x < (H8 ? 1 : 2); x++) {
+            for (int x = 0; x < RX; x++) {
                 const float * q = a.q + (size_t)row_tok[x] * a.q_stride + (size_t)row_head[x] * D;
+                cq[x] = a.scale_log2;
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
                     // the values that the k step's slots of this thread stand for: see the K fragments below
@@ -313,10 +356,7 @@ template <int T, int D, bool H8> __global__ void __launch_bounds__(kDecThreads, 
                     qv[ks][x][2] = live[x] ? __ldg(q + d1) : 0.0f;
                     qv[ks][x][3] = live[x] ? __ldg(q + d1 + 1) : 0.0f;
                 }
-            }
-            if constexpr (T != kBF16) {
-#pragma unroll
-                for (int x = 0; x < (H8 ? 1 : 2); x++) {
+                if constexpr (T != kBF16) {
                     float top = 0.0f;
 #pragma unroll
                     for (int ks = 0; ks < KS; ks++) {
@@ -341,193 +381,230 @@ template <int T, int D, bool H8> __global__ void __launch_bounds__(kDecThreads, 
             }
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                if constexpr (H8) {
-                    split2<T>(qv[ks][0][0], qv[ks][0][1], qa[ks][0][0], qa[ks][0][1]);
-                    split2<T>(qv[ks][0][2], qv[ks][0][3], qa[ks][0][2], qa[ks][0][3]);
-                } else {
 #pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        split2<T>(qv[ks][x][0], qv[ks][x][1], qa[ks][0][x], qa[ks][1][x]);
-                        split2<T>(qv[ks][x][2], qv[ks][x][3], qa[ks][0][2 + x], qa[ks][1][2 + x]);
+                for (int x = 0; x < RX; x++) {
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        uint32_t part[PARTS];
+                        split_pair<T>(qv[ks][x][2 * half], qv[ks][x][2 * half + 1], part);
+                        if constexpr (H8) {
+                            qa[ks][0][2 * half] = part[0];
+                            qa[ks][0][2 * half + 1] = part[1];
+                            if constexpr (PARTS == 3) {
+                                qa[ks][NA - 1][2 * half] = part[2];
+                                qa[ks][NA - 1][2 * half + 1] = 0;
+                            }
+                        } else {
+#pragma unroll
+                            for (int y = 0; y < PARTS; y++) {
+                                qa[ks][y][2 * half + x] = part[y];
+                            }
+                        }
                     }
                 }
             }
         }
-        float o[NT][4];
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        float v[NT * OV]; // o: H8 columns 2t, 2t+1 of row g; otherwise the same of row g + 8 behind them
+        float m[RX], l[RX];
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-            o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+        for (int x = 0; x < RX; x++) {
+            m[x] = -INFINITY;
+            l[x] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < NT * OV; j++) {
+            v[j] = 0.0f;
         }
         const int pos_first = sq.r.n - sq.r.n_row, pos_last = pos_first + sq.r.n_run - 1;
 
-        for (int i = sg.t_begin + warp; i < sg.t_end; i += kDecWarps) {
+        for (int i = sg.t_begin + w_first; i < sg.t_end; i += TEAM) {
             issue();
             cp_async_wait<kDecStages - 1>();
             __syncwarp();
-            const int stage = done % kDecStages;
-            done++;
             const int2 meta = s_meta[warp][stage];
-            const int key0 = meta.x * KT;
+            const int key0 = meta.x;
             const uint32_t sk = ring + stage * kDecStageBytes, sv = sk + kDecStageBytes / 2;
-            // ---- s = q . k
+            stage = stage + 1 == kDecStages ? 0 : stage + 1;
+            // ---- s = q . k, the smallest parts first
             float sc[KT / 8][4];
 #pragma unroll
             for (int n = 0; n < KT / 8; n++) {
                 sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+                uint32_t kb[KS][2];
                 if constexpr (T != kE4M3) {
 #pragma unroll
                     for (int ks = 0; ks < KS; ks += 2) {
-                        uint32_t kb[4];
-                        ldsm4(sk + tile_off<T, ROWB>(n * 8 + (lane & 7), ks * 2 + (lane >> 3)), kb);
-#pragma unroll
-                        for (int y = 0; y < (H8 ? 1 : 2); y++) {
-                            mma16816<T>(sc[n], qa[ks][y], kb[0], kb[1]);
-                            mma16816<T>(sc[n], qa[ks + 1][y], kb[2], kb[3]);
-                        }
+                        uint32_t w[4];
+                        ldsm4(sk + tile_off<T, ROWB>(n * 8 + (lane & 7), ks * 2 + (lane >> 3)), w);
+                        kb[ks][0] = w[0], kb[ks][1] = w[1], kb[ks + 1][0] = w[2], kb[ks + 1][1] = w[3];
                     }
                 } else {
                     // 16 values of key g: words 0..3 are the slots of four k steps
 #pragma unroll
                     for (int c = 0; c < D / 64; c++) {
-                        uint32_t kb[4];
-                        lds128(sk + tile_off<T, ROWB>(n * 8 + g, c * 4 + t4), kb);
+                        uint32_t w[4];
+                        lds128(sk + tile_off<T, ROWB>(n * 8 + g, c * 4 + t4), w);
 #pragma unroll
-                        for (int w = 0; w < 4; w++) {
-                            const uint32_t b0 = e4m3x2_to_f16x2(kb[w]), b1 = e4m3x2_to_f16x2(kb[w] >> 16);
-#pragma unroll
-                            for (int y = 0; y < (H8 ? 1 : 2); y++) {
-                                mma16816<T>(sc[n], qa[c * 4 + w][y], b0, b1);
-                            }
+                        for (int e = 0; e < 4; e++) {
+                            kb[c * 4 + e][0] = e4m3x2_to_f16x2(w[e]);
+                            kb[c * 4 + e][1] = e4m3x2_to_f16x2(w[e] >> 16);
                         }
                     }
                 }
-            }
-            // ---- masks, running maximum
-            if constexpr (H8) { // hi row + lo row
 #pragma unroll
-                for (int n = 0; n < KT / 8; n++) {
+                for (int y = NA - 1; y >= 0; y--) {
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) {
+                        mma16816<T>(sc[n], qa[ks][y], kb[ks][0], kb[ks][1]);
+                    }
+                }
+                if constexpr (H8) { // first part's row + second part's row
                     sc[n][0] += sc[n][2];
                     sc[n][1] += sc[n][3];
                 }
             }
-            constexpr uint32_t kAll = (KT / 16 >= 32) ? ~0u : (1u << (KT / 16)) - 1u;
+            // ---- masks (only tiles on a border), running maximum, p
+            constexpr uint32_t kAll = (1u << GROUPS) - 1u;
             const bool whole = (uint32_t)meta.y == kAll && key0 + KT - 1 <= pos_first &&
                                (a.window == 0 || key0 > pos_last - a.window || key0 + KT <= a.n_sink);
+            float f[RX];
+            if (!whole) {
 #pragma unroll
-            for (int x = 0; x < (H8 ? 1 : 2); x++) {
-                float top = -INFINITY;
-                const int low = a.window ? pos[x] - a.window + 1 : 0;
+                for (int x = 0; x < RX; x++) {
+                    const int low = a.window ? pos[x] - a.window + 1 : 0;
 #pragma unroll
-                for (int n = 0; n < KT / 8; n++) {
+                    for (int n = 0; n < KT / 8; n++) {
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float v = sc[n][2 * x + e] * cq[x];
-                        if (!whole) {
+                        for (int e = 0; e < 2; e++) {
                             const int key = key0 + n * 8 + 2 * t4 + e;
                             const bool seen = key <= pos[x] && (key >= low || key < a.n_sink) && ((meta.y >> (n / 2)) & 1);
-                            v = seen ? v : -INFINITY;
+                            sc[n][2 * x + e] = seen ? sc[n][2 * x + e] : -INFINITY;
                         }
-                        sc[n][2 * x + e] = v;
-                        top = fmaxf(top, v);
-                    }
-                }
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                const float mn = fmaxf(m[x], top);
-                if (__any_sync(~0u, mn > m[x])) {
-                    const float f = mn > m[x] ? exp2f(m[x] - mn) : 1.0f; // m = -inf: 0
-                    l[x] *= f;
-#pragma unroll
-                    for (int j = 0; j < NT; j++) {
-                        if constexpr (H8) {
-                            o[j][0] *= f, o[j][1] *= f, o[j][2] *= f, o[j][3] *= f;
-                        } else {
-                            o[j][2 * x] *= f, o[j][2 * x + 1] *= f;
-                        }
-                    }
-                    m[x] = mn;
-                }
-                const float base = (m[x] == -INFINITY ? 0.0f : m[x]) - kPBias;
-#pragma unroll
-                for (int n = 0; n < KT / 8; n++) {
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const float p = exp2_fast(sc[n][2 * x + e] - base);
-                        sc[n][2 * x + e] = p;
-                        l[x] += p;
                     }
                 }
             }
-            // ---- o += p v
 #pragma unroll
-            for (int kk = 0; kk < KT / 16; kk++) {
-                uint32_t pa[H8 ? 1 : 2][4];
-                if constexpr (H8) {
-                    split2<T>(sc[2 * kk][0], sc[2 * kk][1], pa[0][0], pa[0][1]);
-                    split2<T>(sc[2 * kk + 1][0], sc[2 * kk + 1][1], pa[0][2], pa[0][3]);
-                } else {
+            for (int x = 0; x < RX; x++) {
+                float top = fmaxf(sc[0][2 * x], sc[0][2 * x + 1]);
 #pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        split2<T>(sc[2 * kk][2 * x], sc[2 * kk][2 * x + 1], pa[0][x], pa[1][x]);
-                        split2<T>(sc[2 * kk + 1][2 * x], sc[2 * kk + 1][2 * x + 1], pa[0][2 + x], pa[1][2 + x]);
+                for (int n = 1; n < KT / 8; n++) {
+                    top = fmaxf(top, fmaxf(sc[n][2 * x], sc[n][2 * x + 1]));
+                }
+                top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+                const float mn = fmaxf(m[x], top * cq[x]);
+                f[x] = m[x] == mn ? 1.0f : exp2_fast(m[x] - mn); // nothing seen yet: exp2(-inf) = 0
+                m[x] = mn;
+                const float base = kPBias - (mn == -INFINITY ? 0.0f : mn);
+                float sum = 0.0f;
+#pragma unroll
+                for (int n = 0; n < KT / 8; n++) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float p = exp2_fast(fmaf(sc[n][2 * x + e], cq[x], base));
+                        sc[n][2 * x + e] = p;
+                        sum += p;
                     }
                 }
-                if constexpr (T != kE4M3) {
+                l[x] = fmaf(l[x], f[x], sum);
+            }
+            // ---- o = f o + p v, the smallest parts first
+            uint32_t pa[GROUPS][NA][4];
 #pragma unroll
-                    for (int j = 0; j < NT; j += 2) {
-                        uint32_t vb[4];
-                        ldsm4t(sv + tile_off<T, ROWB>(kk * 16 + (lane & 15), j + (lane >> 4)), vb);
+            for (int kk = 0; kk < GROUPS; kk++) {
 #pragma unroll
-                        for (int y = 0; y < (H8 ? 1 : 2); y++) {
-                            mma16816<T>(o[j], pa[y], vb[0], vb[1]);
-                            mma16816<T>(o[j + 1], pa[y], vb[2], vb[3]);
+                for (int x = 0; x < RX; x++) {
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        uint32_t part[PARTS];
+                        split_pair<T>(sc[2 * kk + half][2 * x], sc[2 * kk + half][2 * x + 1], part);
+                        if constexpr (H8) {
+                            pa[kk][0][2 * half] = part[0];
+                            pa[kk][0][2 * half + 1] = part[1];
+                            if constexpr (PARTS == 3) {
+                                pa[kk][NA - 1][2 * half] = part[2];
+                                pa[kk][NA - 1][2 * half + 1] = 0;
+                            }
+                        } else {
+#pragma unroll
+                            for (int y = 0; y < PARTS; y++) {
+                                pa[kk][y][2 * half + x] = part[y];
+                            }
                         }
                     }
-                } else {
-                    // keys 2t, 2t+1, 2t+8, 2t+9, NT values each from value NT g on: column g of o[j] is value NT g + j
-                    uint32_t w[4][NT / 4];
+                }
+            }
+            constexpr int JC = T == kE4M3 ? 4 : 2; // blocks of eight columns that are taken together
+            // e4m3: keys 2t, 2t+1, 2t+8, 2t+9, NT values each from value NT g on: column g of block j is value NT g + j
+            uint32_t raw[T == kE4M3 ? GROUPS : 1][4][NT / 4];
+            if constexpr (T == kE4M3) {
+#pragma unroll
+                for (int kk = 0; kk < GROUPS; kk++) {
 #pragma unroll
                     for (int y = 0; y < 4; y++) {
                         const int r = kk * 16 + 2 * t4 + (y & 1) + (y >> 1) * 8;
                         if constexpr (D == 128) {
-                            lds128(sv + tile_off<T, ROWB>(r, g), w[y]);
+                            lds128(sv + tile_off<T, ROWB>(r, g), raw[kk][y]);
                         } else {
-                            lds64(sv + tile_off<T, ROWB>(r, g >> 1) + (g & 1) * 8, w[y][0], w[y][1]);
+                            lds64(sv + tile_off<T, ROWB>(r, g >> 1) + (g & 1) * 8, raw[kk][y]);
                         }
                     }
+                }
+            }
 #pragma unroll
-                    for (int q4 = 0; q4 < NT / 4; q4++) {
-                        const uint32_t b0l = __byte_perm(w[0][q4], w[1][q4], 0x5140), b0h = __byte_perm(w[0][q4], w[1][q4], 0x7362);
-                        const uint32_t b1l = __byte_perm(w[2][q4], w[3][q4], 0x5140), b1h = __byte_perm(w[2][q4], w[3][q4], 0x7362);
-                        const uint32_t b0[4] = {e4m3x2_to_f16x2(b0l), e4m3x2_to_f16x2(b0l >> 16), e4m3x2_to_f16x2(b0h), e4m3x2_to_f16x2(b0h >> 16)};
-                        const uint32_t b1[4] = {e4m3x2_to_f16x2(b1l), e4m3x2_to_f16x2(b1l >> 16), e4m3x2_to_f16x2(b1h), e4m3x2_to_f16x2(b1h >> 16)};
+            for (int j = 0; j < NT; j += JC) {
+                float c[JC][4];
+                uint32_t vb[GROUPS][JC][2];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
+                for (int e = 0; e < JC; e++) {
+                    c[e][0] = c[e][1] = c[e][2] = c[e][3] = 0.0f;
+                }
 #pragma unroll
-                            for (int y = 0; y < (H8 ? 1 : 2); y++) {
-                                mma16816<T>(o[q4 * 4 + e], pa[y], b0[e], b1[e]);
-                            }
+                for (int kk = 0; kk < GROUPS; kk++) {
+                    if constexpr (T != kE4M3) {
+                        uint32_t w[4];
+                        ldsm4t(sv + tile_off<T, ROWB>(kk * 16 + (lane & 15), j + (lane >> 4)), w);
+                        vb[kk][0][0] = w[0], vb[kk][0][1] = w[1], vb[kk][1][0] = w[2], vb[kk][1][1] = w[3];
+                    } else {
+                        const uint32_t w[4] = {raw[kk][0][j / 4], raw[kk][1][j / 4], raw[kk][2][j / 4], raw[kk][3][j / 4]};
+                        const uint32_t b0l = __byte_perm(w[0], w[1], 0x5140), b0h = __byte_perm(w[0], w[1], 0x7362);
+                        const uint32_t b1l = __byte_perm(w[2], w[3], 0x5140), b1h = __byte_perm(w[2], w[3], 0x7362);
+                        vb[kk][0][0] = e4m3x2_to_f16x2(b0l), vb[kk][1 % JC][0] = e4m3x2_to_f16x2(b0l >> 16);
+                        vb[kk][2 % JC][0] = e4m3x2_to_f16x2(b0h), vb[kk][3 % JC][0] = e4m3x2_to_f16x2(b0h >> 16);
+                        vb[kk][0][1] = e4m3x2_to_f16x2(b1l), vb[kk][1 % JC][1] = e4m3x2_to_f16x2(b1l >> 16);
+                        vb[kk][2 % JC][1] = e4m3x2_to_f16x2(b1h), vb[kk][3 % JC][1] = e4m3x2_to_f16x2(b1h >> 16);
+                    }
+                }
+#pragma unroll
+                for (int y = NA - 1; y >= 0; y--) {
+#pragma unroll
+                    for (int kk = 0; kk < GROUPS; kk++) {
+#pragma unroll
+                        for (int e = 0; e < JC; e++) {
+                            mma16816<T>(c[e], pa[kk][y], vb[kk][e][0], vb[kk][e][1]);
                         }
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < JC; e++) {
+                    float * o = v + (j + e) * OV;
+                    if constexpr (H8) {
+                        o[0] = fmaf(o[0], f[0], c[e][0] + c[e][2]);
+                        o[1] = fmaf(o[1], f[0], c[e][1] + c[e][3]);
+                    } else {
+                        o[0] = fmaf(o[0], f[0], c[e][0]);
+                        o[1] = fmaf(o[1], f[0], c[e][1]);
+                        o[OV - 2] = fmaf(o[OV - 2], f[RX - 1], c[e][2]);
+                        o[OV - 1] = fmaf(o[OV - 1], f[RX - 1], c[e][3]);
                     }
                 }
             }
             __syncwarp(); // the stage may be filled again
         }
 
-        // ---- join: v[] are the thread's o values, (m, l) of its rows
-        float v[NT * OV];
+        // ---- join
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-            if constexpr (H8) {
-                v[2 * j] = o[j][0] + o[j][2];
-                v[2 * j + 1] = o[j][1] + o[j][3];
-            } else {
-                v[4 * j] = o[j][0], v[4 * j + 1] = o[j][1], v[4 * j + 2] = o[j][2], v[4 * j + 3] = o[j][3];
-            }
-        }
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
+        for (int x = 0; x < RX; x++) {
             l[x] += __shfl_xor_sync(~0u, l[x], 1);
             l[x] += __shfl_xor_sync(~0u, l[x], 2);
         }
@@ -537,95 +614,107 @@ template <int T, int D, bool H8> __global__ void __launch_bounds__(kDecThreads, 
                 p[j * 32 + lane] = v[j];
             }
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
+            for (int x = 0; x < RX; x++) {
                 p[NT * OV * 32 + x * 16 + g] = m[x]; // the same from all four threads of the row
                 p[NT * OV * 32 + x * 16 + 8 + g] = l[x];
             }
         };
         auto take = [&](const float * p) { // joins another part to the thread's
-            float f[2], h[2];
+            float fa[RX], fb[RX];
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
+            for (int x = 0; x < RX; x++) {
                 const float m2 = p[NT * OV * 32 + x * 16 + g], l2 = p[NT * OV * 32 + x * 16 + 8 + g];
                 const float mn = fmaxf(m[x], m2);
-                f[x] = m[x] == mn ? 1.0f : exp2f(m[x] - mn);
-                h[x] = m2 == mn ? 1.0f : exp2f(m2 - mn);
+                fa[x] = m[x] == mn ? 1.0f : exp2_fast(m[x] - mn);
+                fb[x] = m2 == mn ? 1.0f : exp2_fast(m2 - mn);
                 m[x] = mn;
-                l[x] = l[x] * f[x] + l2 * h[x];
+                l[x] = l[x] * fa[x] + l2 * fb[x];
             }
 #pragma unroll
             for (int j = 0; j < NT * OV; j++) {
                 const int x = H8 ? 0 : (j >> 1) & 1;
-                v[j] = v[j] * f[x] + p[j * 32 + lane] * h[x];
+                v[j] = v[j] * fa[x] + p[j * 32 + lane] * fb[x];
             }
         };
-        auto join_warps = [&]() { // warp 0 ends with all
-            __syncthreads();
-            if (warp >= 2) {
-                put(join + (warp - 2) * PART);
-            }
-            __syncthreads();
-            if (warp < 2) {
-                take(join + warp * PART);
-            }
-            __syncthreads();
-            if (warp == 1) {
-                put(join);
-            }
-            __syncthreads();
-            if (warp == 0) {
-                take(join);
+        auto join_team = [&]() { // the team's first warp ends with all
+            if constexpr (TEAM > 1) {
+                __syncthreads();
+                if (warp >= 2) {
+                    put(join + (warp - 2) * PART);
+                }
+                __syncthreads();
+                if (warp < 2) {
+                    take(join + warp * PART);
+                }
+                __syncthreads();
+                if (warp == 1) {
+                    put(join);
+                }
+                __syncthreads();
+                if (warp == 0) {
+                    take(join);
+                }
             }
         };
-        join_warps();
+        const bool lead = TEAM == 1 || warp == 0;
+        join_team();
         bool write = true;
         if (sg.t_end - sg.t_begin != sg.t_unit) {
-            // the unit spans CTAs: its tiles are [u0, u0 + t_unit) of the list
+            // the unit spans workers: its tiles are [u0, u0 + t_unit) of the list
             const long long u0 = at - sg.t_begin;
             auto owner = [&](long long x) { return (int)(((x + 1) * nw - 1) / total); };
             const int b0 = owner(u0), b1 = owner(u0 + sg.t_unit - 1);
-            // of a CTA's two slots the second holds the unit that starts in its share and runs on behind it
-            if (warp == 0) {
-                put(a.parts + ((size_t)blockIdx.x * 2 + (sg.t_begin == 0 ? 1 : 0)) * PART);
+            if (lead) {
+                // of a worker's two slots the second holds the unit that starts in its share and runs on behind it
+                put(a.parts + ((size_t)worker * 2 + (sg.t_begin == 0 ? 1 : 0)) * PART);
                 __threadfence();
                 __syncwarp();
+                uint32_t last = 0;
                 if (lane == 0) {
-                    const int unit = (sg.s * a.kv.n_kv + sg.h) * a.row_blocks + sg.rb;
-                    const uint32_t was = atomicAdd(a.counters + unit, 1u);
-                    s_last = was == (uint32_t)(b1 - b0);
-                    if (s_last) {
-                        a.counters[unit] = 0; // as the next call wants it
+                    uint32_t * counter = a.counters + (sg.s * a.kv.n_kv + sg.h) * a.row_blocks + sg.rb;
+                    last = atomicAdd(counter, 1u) == (uint32_t)(b1 - b0);
+                    if (last) {
+                        *counter = 0; // as the next call wants it
                         __threadfence();
                     }
+                    if constexpr (TEAM > 1) {
+                        s_last = (int)last;
+                    }
                 }
+                write = __shfl_sync(~0u, last, 0);
             }
-            __syncthreads();
-            write = s_last;
+            if constexpr (TEAM > 1) {
+                __syncthreads();
+                write = s_last;
+            }
             if (write) {
-                m[0] = m[1] = -INFINITY;
-                l[0] = l[1] = 0.0f;
+#pragma unroll
+                for (int x = 0; x < RX; x++) {
+                    m[x] = -INFINITY;
+                    l[x] = 0.0f;
+                }
 #pragma unroll
                 for (int j = 0; j < NT * OV; j++) {
                     v[j] = 0.0f;
                 }
-                for (int b = b0 + warp; b <= b1; b += kDecWarps) {
+                for (int b = b0 + w_first; b <= b1; b += TEAM) {
                     take(a.parts + ((size_t)b * 2 + (b == b0 ? 1 : 0)) * PART);
                 }
-                join_warps();
+                join_team();
             }
         }
-        if (write && warp == 0) {
+        if (write && lead) {
 #pragma unroll
-            for (int x = 0; x < (H8 ? 1 : 2); x++) {
+            for (int x = 0; x < RX; x++) {
                 if (live[x]) {
-                    const float f = l[x] > 0.0f || isnan(l[x]) ? a.v_scale / l[x] : 0.0f; // no visible key: zeros
+                    const float r = l[x] > 0.0f || isnan(l[x]) ? a.v_scale / l[x] : 0.0f; // no visible key: zeros
                     float * out = a.out + (size_t)row_tok[x] * a.out_stride + (size_t)row_head[x] * D;
 #pragma unroll
                     for (int j = 0; j < NT; j++) {
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             const int d = T == kE4M3 ? NT * (2 * t4 + e) + j : j * 8 + 2 * t4 + e;
-                            out[d] = v[OV * j + 2 * x + e] * f;
+                            out[d] = v[OV * j + 2 * x + e] * r;
                         }
                     }
                 }
@@ -641,10 +730,9 @@ template <int T, int D, bool H8> __global__ void __launch_bounds__(kDecThreads, 
     cp_async_wait<0>();
 }
 
-template <int T, int D, bool H8> static cudaError_t launch_t(cudaStream_t s, const AttnDev & a, int grid) {
-    constexpr int PART = (D / 8 * (H8 ? 2 : 4) + 1) * 32;
-    constexpr int smem = kDecWarps * kDecStages * kDecStageBytes + 2 * PART * 4;
-    const cudaError_t e = ensure_dynamic_smem((const void *)attn_decode_kernel<T, D, H8>, smem);
+template <int T, int D, bool H8, int TEAM> static cudaError_t launch_t(cudaStream_t s, const AttnDev & a, int grid) {
+    constexpr int smem = kDecWarps * kDecStages * kDecStageBytes + (TEAM > 1 ? 2 * part_floats(D, H8) * 4 : 0);
+    const cudaError_t e = ensure_dynamic_smem((const void *)attn_decode_kernel<T, D, H8, TEAM>, smem);
     if (e != cudaSuccess) {
         return e;
     }
@@ -658,12 +746,14 @@ template <int T, int D, bool H8> static cudaError_t launch_t(cudaStream_t s, con
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attn_decode_kernel<T, D, H8>, a);
+    return cudaLaunchKernelEx(&cfg, attn_decode_kernel<T, D, H8, TEAM>, a);
 }
 
 constexpr int kDecGrid = kSMs * kDecPerSM;
 
 static int dec_rows(int group, int max_q) { return group * max_q <= 8 ? 8 : 16; }
+// With fewer units than this a team of four warps shares a unit's tiles.
+constexpr size_t kTeamUnits = 128;
 
 size_t attn_decode_units(int n_head, int n_kv, int n_seq, int max_q) {
     const int rows = dec_rows(n_head / n_kv, max_q);
@@ -671,16 +761,21 @@ size_t attn_decode_units(int n_head, int n_kv, int n_seq, int max_q) {
 }
 size_t attn_decode_part_bytes(int n_head, int n_kv, int head_dim, int max_q) {
     const int rows = dec_rows(n_head / n_kv, max_q);
-    return (size_t)kDecGrid * 2 * ((size_t)head_dim / 8 * (rows == 8 ? 2 : 4) + 1) * 32 * sizeof(float);
+    return (size_t)kDecGrid * kDecWarps * 2 * part_floats(head_dim, rows == 8) * sizeof(float);
 }
 
 cudaError_t launch_attn_decode(cudaStream_t s, AttnDev a) {
     const int rows = dec_rows(a.group, a.b.max_q);
     a.row_blocks = (a.b.max_q * a.group + rows - 1) / rows;
-    a.min_tiles = kDecWarps;
+    const size_t units = (size_t)a.b.n_seq * a.kv.n_kv * a.row_blocks;
+    const bool team = units < kTeamUnits;
+    a.min_tiles = team ? kDecWarps : 1;
     auto go = [&](auto t, auto d) -> cudaError_t {
         constexpr int T = decltype(t)::value, D = decltype(d)::value;
-        return rows == 8 ? launch_t<T, D, true>(s, a, kDecGrid) : launch_t<T, D, false>(s, a, kDecGrid);
+        if (team) {
+            return rows == 8 ? launch_t<T, D, true, 4>(s, a, kDecGrid) : launch_t<T, D, false, 4>(s, a, kDecGrid);
+        }
+        return rows == 8 ? launch_t<T, D, true, 1>(s, a, kDecGrid) : launch_t<T, D, false, 1>(s, a, kDecGrid);
     };
     auto dim = [&](auto t) {
         return a.kv.head_dim == 64 ? go(t, std::integral_constant<int, 64>{}) : go(t, std::integral_constant<int, 128>{});
