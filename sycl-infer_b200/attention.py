@@ -36,11 +36,12 @@ class kv_cache:
                 raise ValueError(f"kv_cache: the pages of {n} must be contiguous in themselves")
         if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.stride() != v.stride():
             raise ValueError("kv_cache: k and v must agree in shape, type, device and strides")
-        self.k, self.v, self.device = k, v, k.device
+        self.k, self.v, self.device, self.index = k, v, k.device, k.device.index
         self.n_pages, self.n_kv, self.page_size, self.head_dim = k.shape
+        self.kv_width = self.n_kv * self.head_dim
         self.c = KvCache(k.data_ptr(), v.data_ptr(), _TORCH_KV[k.dtype], self.n_pages, self.page_size, self.n_kv, self.head_dim,
                          k.stride(0) if self.n_pages > 1 else self.n_kv * self.page_size * self.head_dim, k_scale, v_scale)
-        self.ref = C.byref(self.c)
+        self.ref, self.raw = C.byref(self.c), bytes(self.c)
 
 
 class kv_batch:

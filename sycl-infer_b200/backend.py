@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from .attention import _int32
-from .capi import MAX_SEGS, AttnOpts, KvCache, Seg, load_lib
+from .capi import MAX_SEGS, AttnOpts, Seg, load_lib
 
 
 def _ptr(t):
@@ -54,13 +54,19 @@ class gemv_seg:
                    _ptr(self.xmeta), _ptr(self.xsumq))
 
 
-def _rows(t, what, device, width=None):
-    """A 2-D fp32 activation view on `device`, one row a token, unit stride within a row: (pointer, row stride)."""
-    if t.dtype != torch.float32 or t.dim() != 2 or t.device != device or (t.numel() and t.stride(1) != 1):
-        raise ValueError(f"{what}: a 2-D float32 tensor on {device} with unit stride within a row is expected")
-    if width is not None and t.shape[1] != width:
-        raise ValueError(f"{what}: rows of {width} values are expected (got {t.shape[1]})")
-    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+_F32 = torch.float32
+
+
+def _rows(t, what, index, n_rows, width=None):
+    """A 2-D fp32 activation view on CUDA device `index`, one row a token, unit stride within a row: (pointer, row
+    stride, row width)."""
+    if t.dtype is not _F32 or t.get_device() != index:
+        raise ValueError(f"{what}: a float32 tensor on cuda:{index} is expected (got {t.dtype} on {t.device})")
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] != n_rows or (width is not None and shape[1] != width) or (stride[1] != 1 and n_rows):
+        raise ValueError(f"{what}: {n_rows} rows" + (f" of {width} values" if width is not None else "") +
+                         f" with unit stride are expected (got shape {tuple(shape)}, strides {stride})")
+    return t.data_ptr(), stride[0] if n_rows > 1 else shape[1], shape[1]
 
 
 def _pack(segs):
@@ -81,6 +87,7 @@ class cuda_backend:
         self.lib = load_lib()
         self.device = torch.device("cuda", device)
         self._stream = stream
+        self._attn, self._rope_append = self.lib.attn, self.lib.rope_append
 
     def name(self):
         return "b200q-cuda"
@@ -211,101 +218,106 @@ class cuda_backend:
         self.lib.check(self.lib.quant_gemv_static(self._s(), arr, n))
 
     # ---- attention side: rotary positions + append, attention over the paged cache, page copies ----
-    def _here(self, *tensors):
-        for t in tensors:
+    def _here(self, *owners):
+        for t in owners:
             if t.device != self.device:
                 raise ValueError(f"a tensor on {t.device} was given to the backend of {self.device}")
+
+    def _call(self, fn, *args):
+        """fn(stream, *args) with this backend's device current: launches go to the current device's context."""
+        index = self.device.index
+        stream = self._stream.cuda_stream if self._stream is not None else torch._C._cuda_getCurrentRawStream(index)
+        if torch._C._cuda_getDevice() == index:
+            rc = fn(stream, *args)
+        else:
+            with torch.cuda.device(index):
+                rc = fn(stream, *args)
+        if rc:
+            self.lib.check(rc)
 
     def rope_table(self, rope):
         """Fills rope.table (n_rot / 2 frequencies in turns a position and the factor, 64 bits); once per model."""
         if rope.table is None:
             rope.table = torch.empty(max(0, rope.c.n_rot) // 2 + 1, dtype=torch.float64, device=self.device)
         self._here(rope.table, *([rope.freq_factors] if rope.freq_factors is not None else []))
-        with torch.cuda.device(self.device):
-            self.lib.check(self.lib.rope_table(self._s(), rope.ref, rope.table.data_ptr()))
+        self._call(self.lib.rope_table, rope.ref, rope.table.data_ptr())
         return rope.table
 
     def rope_append(self, rope, q, k, v, q_out, cache, batch):
         """Rotates q into q_out (may be q itself) and appends the rotated k, and v, to the cache: the newest
         tokens of the batch's sequences.  q, k, v: fp32 rows, views of the q|k|v buffer included; rope None:
         no rotation; q and q_out None: the append alone; k and v None: the rotation of q alone."""
-        if rope is not None and rope.table is None:
-            raise ValueError("rope_append: rope_table() has not been called on this rope_t")
-        self._here(cache, batch, *([rope.table] if rope is not None else []))
-        qp = qs = op = os_ = kp = ks = vp = vs = n_head = 0
+        table = ref = qp = op = kp = vp = None
+        qs = os_ = ks = vs = n_head = 0
+        self._here(cache, batch)
+        if rope is not None:
+            if rope.table is None:
+                raise ValueError("rope_append: rope_table() has not been called on this rope_t")
+            self._here(rope.table)
+            table, ref = rope.table.data_ptr(), rope.ref
         if (q is None) != (q_out is None) or (k is None) != (v is None):
             raise ValueError("rope_append: q goes with q_out, k with v")
-        for t in (q, k, v, q_out):
-            if t is not None and t.shape[0] != batch.n_tok:
-                raise ValueError(f"rope_append: {batch.n_tok} rows are expected (got {t.shape[0]})")
+        index, n = self.device.index, batch.n_tok
         if q is not None:
-            qp, qs = _rows(q, "rope_append: q", self.device)
-            op, os_ = _rows(q_out, "rope_append: q_out", self.device, q.shape[1])
-            n_head, odd = divmod(q.shape[1], cache.head_dim)
+            qp, qs, width = _rows(q, "rope_append: q", index, n)
+            op, os_, _ = _rows(q_out, "rope_append: q_out", index, n, width)
+            n_head, odd = divmod(width, cache.head_dim)
             if odd:
                 raise ValueError("rope_append: the rows of q are not a multiple of head_dim")
         if k is not None:
-            kp, ks = _rows(k, "rope_append: k", self.device, cache.n_kv * cache.head_dim)
-            vp, vs = _rows(v, "rope_append: v", self.device, cache.n_kv * cache.head_dim)
-        call = (self._s(), rope.table.data_ptr() if rope is not None else None, rope.ref if rope is not None else None, qp or None,
-                qs, n_head, kp or None, ks, vp or None, vs, op or None, os_, cache.ref, batch.ref)
-        self._on_device(self.lib.rope_append, call)
+            kp, ks, _ = _rows(k, "rope_append: k", index, n, cache.kv_width)
+            vp, vs, _ = _rows(v, "rope_append: v", index, n, cache.kv_width)
+        if n == 0:
+            return
+        self._call(self._rope_append, table, ref, qp, qs, n_head, kp, ks, vp, vs, op, os_, cache.ref, batch.ref)
 
     def attn(self, q, out, cache, batch, scratch, scale=None, window=0, n_sink=0):
         """Attention of the batch's rows over the cache (b200q_attn): causal, with `window` the newest `window` keys
         and the first n_sink ones only.  scratch: attention.alloc_attn_scratch."""
+        index, n = self.device.index, batch.n_tok
         self._here(cache, batch, scratch)
-        for t in (q, out):
-            if t.shape[0] != batch.n_tok:
-                raise ValueError(f"attn: {batch.n_tok} rows are expected (got {t.shape[0]})")
-        qp, qs = _rows(q, "attn: q", self.device)
-        op, os_ = _rows(out, "attn: out", self.device, q.shape[1])
-        n_head, odd = divmod(q.shape[1], cache.head_dim)
+        qp, qs, width = _rows(q, "attn: q", index, n)
+        op, os_, _ = _rows(out, "attn: out", index, n, width)
+        n_head, odd = divmod(width, cache.head_dim)
         if odd:
             raise ValueError("attn: the rows of q are not a multiple of head_dim")
-        if batch.n_tok == 0:
-            return
         if not scratch.is_contiguous():
             raise ValueError("attn: the scratch must be contiguous")
-        opts = AttnOpts(0.0 if scale is None else float(scale), int(window), int(n_sink))
         if scale is not None and not scale > 0:
             raise ValueError("attn: scale must be above 0 (None: 1 / sqrt(head_dim))")
-        call = (self._s(), qp, qs, n_head, cache.ref, batch.ref, C.byref(opts), op, os_, scratch.data_ptr(),
-                scratch.numel() * scratch.element_size())
-        self._on_device(self.lib.attn, call)
+        if n == 0:
+            return
+        opts = AttnOpts(scale or 0.0, window, n_sink)
+        self._call(self._attn, qp, qs, n_head, cache.ref, batch.ref, C.byref(opts), op, os_, scratch.data_ptr(), scratch.nbytes)
 
     def kv_copy_pages(self, caches, src, dst):
         """Page src[i] -> page dst[i] in every cache of the list (the layers of a model): int32 device
         tensors.  dst entries are distinct and none is a src."""
-        caches = list(caches)
         _int32(src, "kv_copy_pages: src", 1)
         _int32(dst, "kv_copy_pages: dst", 1)
-        if src.numel() != dst.numel() or not caches:
+        n = src.numel()
+        if n != dst.numel() or not caches:
             raise ValueError("kv_copy_pages: as many dst as src, and at least one cache")
-        self._here(src, dst, *caches)
-        arr = (KvCache * len(caches))(*[c.c for c in caches])
-        self._on_device(self.lib.kv_copy_pages, (self._s(), arr, len(caches), src.data_ptr() or None, dst.data_ptr() or None, src.numel()))
+        self._here(src, dst)
+        for c in caches:
+            if c.index != self.device.index:
+                raise ValueError(f"kv_copy_pages: a cache on {c.device} was given to the backend of {self.device}")
+        if n:
+            self._call(self.lib.kv_copy_pages, b"".join([c.raw for c in caches]), len(caches), src.data_ptr(), dst.data_ptr(), n)
 
     def kv_remap(self, table, page_map, out=None):
         """out[s][i] = page_map[table[s][i]] (in place without out); entries outside the map stay."""
         out = table if out is None else out
         for t, n, d in ((table, "table", 2), (out, "out", 2), (page_map, "page_map", 1)):
             _int32(t, f"kv_remap: {n}", d)
+        n_seq, width = table.shape
         if table.shape != out.shape:
             raise ValueError("kv_remap: out has the table's shape")
         self._here(table, page_map, out)
-        if table.numel() == 0:
-            return out
-        stride = lambda t: t.stride(0) if t.shape[0] > 1 else t.shape[1]  # noqa: E731
-        self._on_device(self.lib.kv_remap, (self._s(), table.data_ptr(), stride(table), table.shape[0], table.shape[1],
-                                            page_map.data_ptr(), page_map.numel(), out.data_ptr(), stride(out)))
+        if n_seq and width:
+            self._call(self.lib.kv_remap, table.data_ptr(), table.stride(0) if n_seq > 1 else width, n_seq, width,
+                       page_map.data_ptr(), page_map.numel(), out.data_ptr(), out.stride(0) if n_seq > 1 else width)
         return out
-
-    def _on_device(self, fn, args):
-        if torch.cuda.current_device() == self.device.index:
-            return self.lib.check(fn(*args))
-        with torch.cuda.device(self.device):  # launches go to the current device's context
-            self.lib.check(fn(*args))
 
     # parity instrument (no reference operator: the reference never exposes these sums)
     def i8_block_dots(self, w, type, K, n_rows, x8, TB, t, wd):

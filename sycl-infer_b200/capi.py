@@ -136,7 +136,7 @@ _SIGS = {
     "b200q_rope_append": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, C.c_int, _vp, C.c_int, _vp, C.c_int, _vp, C.c_int, _vp, _vp]),
     "b200q_attn_scratch_bytes": (C.c_size_t, [C.c_int] * 6),
     "b200q_attn": (C.c_int, [_vp, _vp, C.c_int, C.c_int, _vp, _vp, _vp, _vp, C.c_int, _vp, C.c_size_t]),
-    "b200q_kv_copy_pages": (C.c_int, [_vp, C.POINTER(KvCache), C.c_int, _vp, _vp, C.c_int]),
+    "b200q_kv_copy_pages": (C.c_int, [_vp, _vp, C.c_int, _vp, _vp, C.c_int]),
     "b200q_kv_remap": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, _vp, C.c_int, _vp, C.c_int]),
     "b200q_gguf_open": (C.c_int, [C.c_char_p, C.POINTER(_vp)]),
     "b200q_gguf_close": (None, [_vp]),
