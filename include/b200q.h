@@ -363,7 +363,7 @@ typedef struct b200q_kv_batch {
     const int32_t * q_start;    /* device, n_seq + 1 entries, non-decreasing, first >= 0, last <= n_tok */
     const int32_t * kv_len;     /* device, n_seq entries */
     int32_t table_stride;       /* entries from one sequence's table to the next one's */
-    int32_t n_seq;
+    int32_t n_seq;              /* up to 4096 */
     int32_t n_tok;              /* rows of the activation buffers */
     int32_t max_q;              /* no sequence has more rows than this (further rows are left as they were) */
 } b200q_kv_batch;

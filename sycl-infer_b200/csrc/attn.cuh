@@ -20,31 +20,55 @@ struct AttnDev {
     uint32_t * counters; // scratch: arrivals a unit, zero between calls
     int32_t row_blocks;  // row blocks of a (sequence, KV head) at most
     int32_t min_tiles;   // tiles that a CTA gets at least
+    int32_t vec;         // rows of q and out can be read and written 16 bytes at a time
 };
 
+// More query rows of a (sequence, KV head) than this take the prompt kernel (attn_prompt.cu).
+constexpr int kDecodeRows = 16;
+constexpr int kMaxSeqs = 4096; // of one step
+
+cudaError_t launch_attn_prompt(cudaStream_t s, AttnDev a);
+size_t attn_prompt_units(int n_head, int n_kv, int n_seq, int max_q);
+size_t attn_prompt_part_bytes(int head_dim);
+cudaError_t read_attn_prompt_status(int * status, bool clear);
 cudaError_t launch_attn_decode(cudaStream_t s, AttnDev a);
 size_t attn_decode_units(int n_head, int n_kv, int n_seq, int max_q);
 size_t attn_decode_part_bytes(int n_head, int n_kv, int head_dim, int max_q);
 
 #ifdef __CUDACC__
 
-// Tiles of `kt` keys that some row of a sequence sees: those of the first n_sink keys, then those from the oldest
-// key in any row's window to the newest.  At least one, so that rows that see nothing are still written.
+// Tiles of `kt` keys that some of a unit's rows see, whose first row is at position pos_first and whose last key is n - 1:
+// those of the first n_sink keys, then those from the oldest key in any row's window to the newest.  At least one,
+// so that rows that see nothing are still written.
 struct KeyTiles {
+    int n;          // keys 0 .. n-1 exist for the unit
     int oldest;     // oldest key in any row's window
     int sink_tiles; // tiles of the list that belong to the sinks alone
     int t_lo;       // tile of `oldest`
     int count;
 };
-__device__ __forceinline__ KeyTiles key_tiles(const SeqRows & r, int kt, int window, int n_sink) {
+__device__ __forceinline__ KeyTiles key_tiles(int pos_first, int n, int kt, int window, int n_sink) {
     KeyTiles k;
-    const int pos_first = r.n - r.n_row;
+    k.n = n;
     k.oldest = window ? max(0, pos_first - window + 1) : 0;
-    k.oldest = min(k.oldest, r.n);
+    k.oldest = min(k.oldest, n);
     k.t_lo = k.oldest / kt;
-    k.sink_tiles = min((min(n_sink, r.n) + kt - 1) / kt, k.t_lo);
-    k.count = max(1, k.sink_tiles + (r.n + kt - 1) / kt - k.t_lo);
+    k.sink_tiles = min((min(n_sink, n) + kt - 1) / kt, k.t_lo);
+    k.count = max(1, k.sink_tiles + (n + kt - 1) / kt - k.t_lo);
     return k;
+}
+// Which of the 16 keys from k0 on some row sees, as bits.
+__device__ __forceinline__ uint32_t keys_seen(const KeyTiles & k, int k0, int n_sink) {
+    if (k0 >= k.n) {
+        return 0;
+    }
+    uint32_t seen = k0 + 16 <= k.n ? 0xFFFFu : 0xFFFFu >> (k0 + 16 - k.n);
+    if (k0 < k.oldest) {
+        uint32_t keep = k.oldest - k0 >= 16 ? 0u : 0xFFFFu << (k.oldest - k0);
+        keep |= n_sink - k0 >= 16 ? 0xFFFFu : (n_sink > k0 ? 0xFFFFu >> (16 - (n_sink - k0)) : 0u);
+        seen &= keep;
+    }
+    return seen;
 }
 __device__ __forceinline__ int key_tile(const KeyTiles & k, int i) { return i < k.sink_tiles ? i : i - k.sink_tiles + k.t_lo; }
 

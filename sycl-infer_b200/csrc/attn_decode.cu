@@ -102,7 +102,7 @@ struct SeqTiles {
 template <int KT, int ROWS> __device__ __forceinline__ SeqTiles seq_tiles(const AttnDev & a, int s) {
     SeqTiles q;
     q.r = seq_rows(a.b, a.kv.page_shift, s);
-    q.k = key_tiles(q.r, KT, a.window, a.n_sink);
+    q.k = key_tiles(q.r.n - q.r.n_row, q.r.n, KT, a.window, a.n_sink);
     q.blocks = (q.r.n_run * a.group + ROWS - 1) / ROWS;
     return q;
 }
@@ -265,18 +265,14 @@ __global__ void __launch_bounds__(kDecThreads, kDecPerSM) attn_decode_kernel(con
         uint32_t seen = 0;
         if (lane < GROUPS) {
             const int k0 = key0 + lane * 16;
-            if (k0 < pq.r.n && (k0 + 15 >= pq.k.oldest || k0 < a.n_sink)) {
+            seen = keys_seen(pq.k, k0, a.n_sink);
+            if (seen) {
                 const int page = a.b.page_table[(size_t)ps.s * a.b.table_stride + (k0 >> a.kv.page_shift)];
                 if (page >= 0 && page < a.kv.n_pages) {
                     src = (unsigned long long)page * a.kv.page_bytes +
                           (((unsigned long long)ps.h << a.kv.page_shift) + (k0 & ((1 << a.kv.page_shift) - 1))) * ROWB;
-                    seen = k0 + 16 <= pq.r.n ? 0xFFFFu : 0xFFFFu >> (k0 + 16 - pq.r.n);
-                    if (k0 < pq.k.oldest) {
-                        uint32_t keep = pq.k.oldest - k0 >= 16 ? 0u : 0xFFFFu << (pq.k.oldest - k0);
-                        keep |= a.n_sink - k0 >= 16 ? 0xFFFFu : (a.n_sink > k0 ? 0xFFFFu >> (16 - (a.n_sink - k0)) : 0u);
-                        seen &= keep;
-                    }
                 } else {
+                    seen = 0;
                     atomicExch(&g_attn_status, B200Q_EINVAL);
                 }
             }

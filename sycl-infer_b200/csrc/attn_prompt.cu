@@ -1,0 +1,814 @@
+// Attention of many new tokens per sequence (prompts, chunks of prompts, long drafts) over the paged cache.
+//
+// The same sums as attn_decode.cu with the query rows in tiles of 128 on the fifth-generation tensor cores.
+//
+// * Units.  A unit is (sequence, KV head, 256 query rows): the rows are (token, query head of the group) pairs, so that K
+//   and V are read once for all heads that share them, and run as two tiles of 128 rows that take turns: while the
+//   tensor core multiplies for one, the other's softmax runs.  The units' key tiles of 128 in order form one list of
+//   which each of the 148 CTAs takes an equal share; what the causal mask or the window hides from a whole unit is not in
+//   the list.  A unit that spans CTAs is joined over the scratch by the CTA that finishes last, in order.
+// * Accuracy.  q and p are split into two 16-bit parts (22 bits for fp16 and e4m3 caches, 16 for bf16), so both products take
+//   twice the tensor work, which is what bounds the kernel: 4 x 128 x 128 x D multiply-adds a tile against 4096 a clock.
+//   The tensor cores' sums drop bits towards zero at every step; each tile's p v therefore starts from zero in tensor
+//   memory, low parts first, and the softmax threads add it to o in registers, rounded, with the factor of the new
+//   maximum.  No accumulator is ever rescaled in tensor memory.
+// * Roles.  Warps 0-3 and 4-7: softmax of the two tiles, a thread a row (o: D registers); warp 8: one thread issues the
+//   products; warps 9-11 bring K and V into shared memory in the 128-byte swizzled form (16-bit caches by asynchronous
+//   copies, e4m3 widened to fp16 on the way), rows that nobody sees as zeros.
+//   Tensor memory: s of both tiles (128 columns each; p's two parts take the place of s as it is consumed), p v of both.
+// * Every wait is bounded; when one runs out the status word is set and all roles run to their end without waiting.
+#include "async.cuh"
+#include "attn.cuh"
+
+namespace b200q {
+
+__device__ int g_attn_prompt_status = 0;
+
+constexpr int kPrThreads = 384;
+constexpr int kPrRows = 256; // rows of a unit
+constexpr int kPrKeys = 128; // keys of a tile
+constexpr int kPrProducers = 96;
+constexpr int kPrHeader = 512;
+
+__host__ __device__ constexpr int pr_slots(int dim) { return dim == 128 ? 3 : 6; }
+__host__ __device__ constexpr int pr_tile_bytes(int dim) { return 128 * dim * 2; } // 128 rows of 16-bit values
+__host__ __device__ constexpr int pr_smem(int dim) { return (4 + pr_slots(dim)) * pr_tile_bytes(dim) + kPrHeader + 1024; }
+// floats that a CTA leaves of one 128-row tile: o by column, then m and l
+__host__ __device__ constexpr int pr_part_floats(int dim) { return (dim + 2) * 128; }
+
+// D[tmem] (+)= A B, 16-bit operands, fp32 sums; issued by one thread.  A from shared or from tensor memory.
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t * u = reinterpret_cast<uint32_t *>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
+                   "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]),
+                   "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]),
+                   "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&u)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+                 "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+                 "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand descriptor, 128-byte swizzle: rows of 128 bytes in atoms of eight, `lbo` and `sbo` the byte
+// distances between atoms (see the uses).
+__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+    d |= (uint64_t)((lbo >> 4) & 0x3FFF) << 16;
+    d |= (uint64_t)((sbo >> 4) & 0x3FFF) << 32;
+    d |= (uint64_t)1 << 46; // descriptor version of this architecture
+    d |= (uint64_t)2 << 61; // 128-byte swizzle
+    return d;
+}
+// kind::f16: fp32 sums, fp16 or bf16 operands, A K-major, B K-major or (b_mn) N-major, M = 128
+__device__ __forceinline__ uint32_t idesc_f16(bool bf16, bool b_mn, int N) {
+    uint32_t d = 0;
+    d |= 1u << 4;
+    d |= (uint32_t)bf16 << 7;
+    d |= (uint32_t)bf16 << 10;
+    d |= (uint32_t)b_mn << 16;
+    d |= (uint32_t)(N >> 3) << 17;
+    d |= (uint32_t)(128 >> 4) << 24;
+    return d;
+}
+// 16-byte chunk c of row r in a tile of 128 rows of 16-bit values: blocks of 64 values, 128 bytes a row, swizzled
+__device__ __forceinline__ uint32_t sw128_off(int r, int c) {
+    return (uint32_t)((c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+// the 128 softmax threads of a tile
+__device__ __forceinline__ void tile_sync(int t) {
+    if (t == 0) {
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+    } else {
+        asm volatile("bar.sync 2, 128;" ::: "memory");
+    }
+}
+
+// A unit's rows and keys.
+struct PromptUnit {
+    SeqRows r;
+    KeyTiles k;
+    int blocks; // row blocks of the sequence
+    int rows;   // rows of this block, at most kPrRows
+    int row0;   // first row among the sequence's (token, head) rows
+};
+struct PromptSeg {
+    int s, h, rb;
+    int t_begin, t_end;
+};
+
+struct PromptBars {
+    uint32_t q_full, s_full, p_full, kv_full, kv_empty, drain; // arrays of 8-byte barriers
+};
+
+template <int T, int D> struct Prompt {
+    static constexpr int TILE = pr_tile_bytes(D), SLOTS = pr_slots(D), KS = D / 16;
+    static constexpr bool BF = T == kBF16;
+    static constexpr float BIAS = BF ? 0.0f : 14.0f;
+
+    const AttnDev & a;
+    uint32_t base;    // shared memory: Q[tile][part], K/V slots, header
+    uint32_t hdr;
+    uint32_t tmem;
+    volatile int * fail;
+    PromptBars bars;
+
+    __device__ __forceinline__ uint32_t q_addr(int tile, int part) const { return base + (tile * 2 + part) * TILE; }
+    __device__ __forceinline__ uint32_t slot_addr(int slot) const { return base + (4 + slot) * TILE; }
+
+    // a bounded wait; after one has run out nobody waits any more
+    __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity) const {
+        if (*fail) {
+            return;
+        }
+        if (!mbar_wait(bar, parity, &g_attn_prompt_status)) {
+            *fail = 1;
+        }
+    }
+
+    __device__ __forceinline__ PromptUnit unit(int s, int rb) const {
+        PromptUnit u;
+        u.r = seq_rows(a.b, a.kv.page_shift, s);
+        const int all = u.r.n_run * a.group;
+        u.blocks = (all + kPrRows - 1) / kPrRows;
+        u.row0 = rb * kPrRows;
+        u.rows = min(all - u.row0, kPrRows);
+        const int first = u.r.n - u.r.n_row;
+        const int pos0 = first + u.row0 / a.group, pos1 = first + (u.row0 + max(u.rows, 1) - 1) / a.group;
+        u.k = key_tiles(pos0, min(u.r.n, max(pos1 + 1, 0)), kPrKeys, a.window, a.n_sink);
+        return u;
+    }
+    // to the next unit of the share, `left` tiles still to come (> 0)
+    __device__ __forceinline__ void advance(PromptSeg & x, long long left, PromptUnit & u) const {
+        // heads innermost: neighbouring CTAs read neighbouring heads of the same pages
+        if (++x.h == a.kv.n_kv) {
+            x.h = 0;
+            if (++x.rb >= u.blocks) {
+                x.rb = 0;
+                do {
+                    x.s++;
+                    u = unit(x.s, 0);
+                } while (u.blocks == 0 && x.s + 1 < a.b.n_seq);
+            } else {
+                u = unit(x.s, x.rb);
+            }
+        }
+        x.t_begin = 0;
+        x.t_end = (int)(left < u.k.count ? left : u.k.count);
+    }
+
+    // ---- warp 8, one thread: the products
+    __device__ void multiply(PromptSeg x, PromptUnit u, long long left) const {
+        const uint32_t id_qk = idesc_f16(BF, false, kPrKeys), id_pv = idesc_f16(BF, true, D);
+        uint32_t p_par = 0, q_par = 0, item = 0; // a bit a tile: the phase that is waited for
+        auto s_cols = [&](int t) { return tmem + (uint32_t)t * 128; };
+        auto o_cols = [&](int t) { return tmem + 256 + (uint32_t)t * 128; };
+        // the loops stay loops: a product takes longer than its issue, and unrolled descriptors would spill
+        auto scores = [&](int t, uint32_t slot) { // s = q k: low part first
+            const uint64_t kd = smem_desc_sw128(slot_addr((int)slot), 16, 1024);
+            uint32_t accumulate = 0;
+#pragma unroll 1
+            for (int part = 1; part >= 0; part--) {
+                const uint64_t qd = smem_desc_sw128(q_addr(t, part), 16, 1024);
+#pragma unroll 1
+                for (int ks = 0; ks < KS; ks++) { // 16 values: 32 bytes of a 128-byte row, then the next block of 64
+                    const uint64_t off = (uint64_t)(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
+                    mma_f16_ss(s_cols(t), qd + off, kd + off, id_qk, accumulate);
+                    accumulate = 1;
+                }
+            }
+        };
+        auto values = [&](int t, uint32_t slot) { // o = p v: low part first
+            // V as stored is N-major: blocks of 64 values 16384 bytes apart, groups of eight keys 1024
+            const uint64_t vd = smem_desc_sw128(slot_addr((int)slot), 16384, 1024);
+            uint32_t accumulate = 0;
+#pragma unroll 1
+            for (int part = 1; part >= 0; part--) {
+#pragma unroll 1
+                for (int ks = 0; ks < kPrKeys / 16; ks++) {
+                    const uint32_t p = s_cols(t) + (uint32_t)((ks >> 1) * 32 + (ks & 1) * 8 + part * 16);
+                    mma_f16_ts(o_cols(t), p, vd + (uint64_t)(ks * (2048 >> 4)), id_pv, accumulate);
+                    accumulate = 1;
+                }
+            }
+        };
+        auto full = [&](uint32_t it) { wait(bars.kv_full + 8 * (it % SLOTS), (it / SLOTS) & 1); };
+        auto release = [&](uint32_t it) { mma_commit(bars.kv_empty + 8 * (it % SLOTS)); };
+        for (;;) {
+            const int tiles = u.rows > 128 ? 2 : 1, n = x.t_end - x.t_begin;
+            // items of this segment: K 0, V 0, K 1, V 1, ...
+            full(item);
+            tc_fence_after();
+            for (int t = 0; t < tiles; t++) {
+                wait(bars.q_full + 8 * t, (q_par >> t) & 1);
+                q_par ^= 1u << t;
+                tc_fence_after();
+                scores(t, item % SLOTS);
+                mma_commit(bars.s_full + 8 * t);
+            }
+            release(item);
+            for (int j = 0; j < n; j++) {
+                const uint32_t iv = item + 2 * j + 1, ik = iv + 1;
+                for (int t = 0; t < tiles; t++) {
+                    wait(bars.p_full + 8 * t, (p_par >> t) & 1);
+                    p_par ^= 1u << t;
+                    if (t == 0) {
+                        full(iv);
+                    }
+                    tc_fence_after();
+                    values(t, iv % SLOTS);
+                    if (j + 1 < n) {
+                        if (t == 0) {
+                            full(ik);
+                            tc_fence_after();
+                        }
+                        scores(t, ik % SLOTS);
+                    }
+                    mma_commit(bars.s_full + 8 * t);
+                }
+                release(iv);
+                if (j + 1 < n) {
+                    release(ik);
+                }
+            }
+            item += 2 * n;
+            left -= n;
+            if (left <= 0) {
+                break;
+            }
+            advance(x, left, u);
+        }
+        mma_commit(bars.drain); // tensor memory is given back only when every product is done
+        mbar_wait(bars.drain, 0, &g_attn_prompt_status);
+    }
+
+    // ---- warps 9-11: K and V into shared memory
+    __device__ void produce(PromptSeg x, PromptUnit u, long long left) const {
+        constexpr int EB = KvElem<T>::BYTES, ROWB = D * EB;
+        constexpr int PIECES = kPrKeys * ROWB / 512;    // runs of 32 chunks of 16 bytes: one a warp
+        constexpr int PER_GROUP = 16 * ROWB / 512;      // of a group of 16 keys
+        constexpr int MINE = (PIECES + 2) / 3;
+        constexpr int CPR = ROWB / 16;
+        const int w = (int)(threadIdx.x >> 5) - 9, lane = threadIdx.x & 31;
+        uint32_t item = 0;
+        int pending = -1; // slot whose copies are in flight
+        volatile int * meta = reinterpret_cast<volatile int *>(__cvta_shared_to_generic(hdr + 256));
+        uint32_t tile_n = 0;
+        auto flush = [&](bool all) {
+            if (pending >= 0) {
+                if (all) {
+                    cp_async_wait<0>();
+                } else {
+                    cp_async_wait<1>();
+                }
+                fence_proxy_async();
+                mbar_arrive(bars.kv_full + 8 * pending);
+                pending = -1;
+            }
+        };
+        auto ready = [&](uint32_t bar, uint32_t parity) {
+            uint32_t ok;
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                         : "=r"(ok)
+                         : "r"(bar), "r"(parity)
+                         : "memory");
+            return __all_sync(~0u, ok != 0);
+        };
+        // the tile's groups of 16 keys, one a lane: where its rows lie and which of them are seen
+        auto look = [&](int tile, unsigned long long & src, uint32_t & seen) {
+            src = 0;
+            seen = 0;
+            if (lane < kPrKeys / 16) {
+                const int k0 = tile * kPrKeys + lane * 16;
+                seen = keys_seen(u.k, k0, a.n_sink);
+                if (seen) {
+                    const int page = a.b.page_table[(size_t)x.s * a.b.table_stride + (k0 >> a.kv.page_shift)];
+                    if (page >= 0 && page < a.kv.n_pages) {
+                        src = (unsigned long long)page * a.kv.page_bytes +
+                              (((unsigned long long)x.h << a.kv.page_shift) + (k0 & ((1 << a.kv.page_shift) - 1))) * ROWB;
+                    } else {
+                        seen = 0;
+                        atomicExch(&g_attn_prompt_status, B200Q_EINVAL);
+                    }
+                }
+            }
+        };
+        for (;;) {
+            for (int j = x.t_begin; j < x.t_end; j++) {
+                unsigned long long src;
+                uint32_t seen;
+                look(key_tile(u.k, j), src, seen);
+                const uint32_t valid = __ballot_sync(~0u, seen != 0);
+                if (w == 0 && lane == 0) {
+                    meta[tile_n & 7] = (int)valid;
+                }
+                tile_n++;
+                for (int kv = 0; kv < 2; kv++, item++) {
+                    const int slot = (int)(item % SLOTS);
+                    const uint32_t bar = bars.kv_empty + 8 * slot, parity = ((item / SLOTS) & 1) ^ 1;
+                    if (pending >= 0 && !ready(bar, parity)) {
+                        flush(true);
+                    }
+                    wait(bar, parity);
+                    __syncwarp();
+                    const uint8_t * pool = kv ? a.kv.v : a.kv.k;
+                    const uint32_t dst = slot_addr(slot);
+                    if constexpr (T != kE4M3) {
+#pragma unroll 4
+                        for (int i = w; i < PIECES; i += 3) {
+                            const int gr = i / PER_GROUP;
+                            const unsigned long long off = __shfl_sync(~0u, src, gr) + (i % PER_GROUP) * 512 + lane * 16;
+                            const uint32_t rows = __shfl_sync(~0u, seen, gr);
+                            const int r = i * (32 / CPR) + lane / CPR;
+                            const bool take = (rows >> (r & 15)) & 1;
+                            const uint32_t to = dst + sw128_off(r, lane % CPR);
+                            const int n = take ? 16 : 0;
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(take ? pool + off : pool), "r"(n)
+                                         : "memory");
+                        }
+                        cp_async_commit();
+                        flush(false);
+                        pending = slot;
+                    } else {
+                        uint4 raw[MINE];
+#pragma unroll
+                        for (int q = 0; q < MINE; q++) {
+                            const int i = w + 3 * q;
+                            const int gr = min(i / PER_GROUP, kPrKeys / 16 - 1);
+                            const unsigned long long off = __shfl_sync(~0u, src, gr) + (i % PER_GROUP) * 512 + lane * 16;
+                            const uint32_t rows = __shfl_sync(~0u, seen, gr);
+                            const int r = i * (32 / CPR) + lane / CPR;
+                            raw[q] = make_uint4(0, 0, 0, 0);
+                            if (i < PIECES && ((rows >> (r & 15)) & 1)) {
+                                raw[q] = __ldg(reinterpret_cast<const uint4 *>(pool + off));
+                            }
+                        }
+#pragma unroll
+                        for (int q = 0; q < MINE; q++) {
+                            const int i = w + 3 * q;
+                            if (i < PIECES) {
+                                const int r = i * (32 / CPR) + lane / CPR, c = lane % CPR * 2;
+                                sts128(dst + sw128_off(r, c), e4m3x2_to_f16x2(raw[q].x), e4m3x2_to_f16x2(raw[q].x >> 16),
+                                       e4m3x2_to_f16x2(raw[q].y), e4m3x2_to_f16x2(raw[q].y >> 16));
+                                sts128(dst + sw128_off(r, c + 1), e4m3x2_to_f16x2(raw[q].z), e4m3x2_to_f16x2(raw[q].z >> 16),
+                                       e4m3x2_to_f16x2(raw[q].w), e4m3x2_to_f16x2(raw[q].w >> 16));
+                            }
+                        }
+                        fence_proxy_async();
+                        mbar_arrive(bars.kv_full + 8 * slot);
+                    }
+                }
+            }
+            left -= x.t_end - x.t_begin;
+            if (left <= 0) {
+                break;
+            }
+            advance(x, left, u);
+        }
+        flush(true);
+    }
+
+    // ---- warps 0-3 and 4-7: softmax, a thread a row of its tile
+    __device__ void softmax(PromptSeg x, PromptUnit u, long long left, long long at, long long each, long long more) const {
+        const int tid = threadIdx.x & 127, t = (int)(threadIdx.x >> 7);
+        const uint32_t lanes = (uint32_t)(32 * ((threadIdx.x >> 5) & 3)) << 16;
+        const uint32_t s_cols = tmem + lanes + (uint32_t)t * 128, o_cols = tmem + lanes + 256 + (uint32_t)t * 128;
+        const volatile int * meta = reinterpret_cast<const volatile int *>(__cvta_shared_to_generic(hdr + 256));
+        volatile int * last = reinterpret_cast<volatile int *>(__cvta_shared_to_generic(hdr + 320)) + t;
+        uint32_t s_n = 0, tile_n = 0;
+        for (;;) {
+            const int n = x.t_end - x.t_begin;
+            const bool mine = t == 0 || u.rows > 128; // the second tile may be empty
+            if (mine) {
+                const int r = u.row0 + t * 128 + tid, r_end = u.row0 + u.rows;
+                const bool live = r < r_end;
+                const int first = u.r.n - u.r.n_row;
+                const int tok = live ? r / a.group : 0, head = x.h * a.group + (live ? r - tok * a.group : 0);
+                const int pos = live ? first + tok : -1;
+                const int pos_min = first + (u.row0 + t * 128) / a.group;
+                const int pos_max = first + (min(u.row0 + t * 128 + 127, r_end - 1)) / a.group;
+                const float * q = a.q + (size_t)(u.r.row0 + tok) * a.q_stride + (size_t)head * D;
+                // q in two parts to shared memory
+                float cq = a.scale_log2;
+                float up = 1.0f;
+                auto q4 = [&](int d) {
+                    if (!live) {
+                        return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    }
+                    if (a.vec) {
+                        return __ldg(reinterpret_cast<const float4 *>(q + d));
+                    }
+                    return make_float4(__ldg(q + d), __ldg(q + d + 1), __ldg(q + d + 2), __ldg(q + d + 3));
+                };
+                if constexpr (!BF) {
+                    float top = 0.0f;
+#pragma unroll 8
+                    for (int d = 0; d < D; d += 4) {
+                        const float4 v = q4(d);
+                        top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+                    }
+                    const int e = pow2_to_top(top);
+                    up = exp2_int(e);
+                    cq *= exp2_int(-e);
+                }
+#pragma unroll 4
+                for (int c = 0; c < D / 8; c++) {
+                    const float4 v = q4(c * 8), w = q4(c * 8 + 4);
+                    uint32_t p0[2], p1[2], p2[2], p3[2];
+                    split_pair<T>(v.x * up, v.y * up, p0);
+                    split_pair<T>(v.z * up, v.w * up, p1);
+                    split_pair<T>(w.x * up, w.y * up, p2);
+                    split_pair<T>(w.z * up, w.w * up, p3);
+                    sts128(q_addr(t, 0) + sw128_off(tid, c), p0[0], p1[0], p2[0], p3[0]);
+                    sts128(q_addr(t, 1) + sw128_off(tid, c), p0[1], p1[1], p2[1], p3[1]);
+                }
+                fence_proxy_async();
+                mbar_arrive(bars.q_full + 8 * t);
+
+                float o[D];
+#pragma unroll
+                for (int d = 0; d < D; d++) {
+                    o[d] = 0.0f;
+                }
+                float m = -INFINITY, l = 0.0f, f = 1.0f;
+                const int low = a.window ? pos - a.window + 1 : 0;
+                auto add_o = [&]() { // o = o f + the tile's p v
+#pragma unroll
+                    for (int c = 0; c < D / 32; c++) {
+                        float v[32];
+                        tmem_ld32(o_cols + 32 * c, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            o[32 * c + i] = fmaf(o[32 * c + i], f, v[i]);
+                        }
+                    }
+                };
+                for (int j = 0; j < n; j++) {
+                    wait(bars.s_full + 8 * t, s_n & 1);
+                    s_n++;
+                    __syncwarp();
+                    tc_fence_after();
+                    const int key0 = key_tile(u.k, x.t_begin + j) * kPrKeys;
+                    const uint32_t valid = (uint32_t)meta[(tile_n + j) & 7];
+                    const bool whole = valid == 0xFFu && key0 + kPrKeys - 1 <= pos_min &&
+                                       (a.window == 0 || key0 > pos_max - a.window || key0 + kPrKeys <= a.n_sink);
+                    const int c_hi = pos - key0, c_lo = low - key0, c_sink = a.n_sink - key0;
+                    auto load = [&](int c, float (&v)[32]) {
+                        tmem_ld32(s_cols + 32 * c, v);
+                        tmem_ld_wait();
+                        if (!whole) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++) {
+                                const int col = 32 * c + i;
+                                const bool seen = col <= c_hi && (col >= c_lo || col < c_sink) && ((valid >> (2 * c + i / 16)) & 1);
+                                v[i] = seen ? v[i] : -INFINITY;
+                            }
+                        }
+                    };
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        float v[32];
+                        load(c, v);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            top = fmaxf(top, fmaxf(v[i], v[i + 1]));
+                        }
+                    }
+                    const float mn = fmaxf(m, top * cq);
+                    const float f_new = m == mn ? 1.0f : exp2_fast(m - mn);
+                    const float off = BIAS - (mn == -INFINITY ? 0.0f : mn);
+                    m = mn;
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        float v[32];
+                        load(c, v);
+                        uint32_t hi[16], lo[16];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const float p0 = exp2_fast(fmaf(v[i], cq, off)), p1 = exp2_fast(fmaf(v[i + 1], cq, off));
+                            sum[i & 2] += p0;
+                            sum[(i & 2) + 1] += p1;
+                            uint32_t part[2];
+                            split_pair<T>(p0, p1, part);
+                            hi[i / 2] = part[0];
+                            lo[i / 2] = part[1];
+                        }
+                        tmem_st16(s_cols + 32 * c, hi); // over the 32 columns of s that were just read
+                        tmem_st16(s_cols + 32 * c + 16, lo);
+                    }
+                    l = fmaf(l, f_new, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                    if (j > 0) {
+                        add_o(); // of the tile before: complete, its commit came before this tile's s
+                    }
+                    f = f_new;
+                    tmem_st_wait();
+                    tc_fence_before();
+                    mbar_arrive(bars.p_full + 8 * t);
+                }
+                wait(bars.s_full + 8 * t, s_n & 1);
+                s_n++;
+                __syncwarp();
+                tc_fence_after();
+                add_o();
+                tc_fence_before();
+
+                bool write = true;
+                if (n != u.k.count) {
+                    // the unit spans CTAs: its tiles are [u0, u0 + count) of the list
+                    const long long u0 = at - x.t_begin;
+                    auto owner = [&](long long y) { // the CTA whose share holds tile y
+                        return (int)(y < more * (each + 1) ? y / (each + 1) : more + (y - more * (each + 1)) / each);
+                    };
+                    const int b0 = owner(u0), b1 = owner(u0 + u.k.count - 1);
+                    auto part = [&](int b, bool second) {
+                        return a.parts + ((size_t)(b * 2 + (second ? 1 : 0)) * 2 + t) * pr_part_floats(D) + tid;
+                    };
+                    // of a CTA's two places the second holds the unit that starts in its share and runs on behind it
+                    float * mine_p = part((int)blockIdx.x, x.t_begin == 0);
+#pragma unroll
+                    for (int d = 0; d < D; d++) {
+                        mine_p[d * 128] = o[d];
+                    }
+                    mine_p[D * 128] = m;
+                    mine_p[(D + 1) * 128] = l;
+                    __threadfence();
+                    tile_sync(t);
+                    if (tid == 0) {
+                        uint32_t * counter = a.counters + ((size_t)(x.s * a.kv.n_kv + x.h) * a.row_blocks + x.rb) * 2 + t;
+                        const bool end = atomicAdd(counter, 1u) == (uint32_t)(b1 - b0);
+                        if (end) {
+                            *counter = 0; // as the next call wants it
+                        }
+                        __threadfence();
+                        *last = end;
+                    }
+                    tile_sync(t);
+                    write = *last;
+                    if (write) {
+                        m = -INFINITY;
+                        for (int b = b0; b <= b1; b++) {
+                            m = fmaxf(m, __ldcg(part(b, b == b0) + D * 128));
+                        }
+                        l = 0.0f;
+#pragma unroll
+                        for (int d = 0; d < D; d++) {
+                            o[d] = 0.0f;
+                        }
+                        for (int b = b0; b <= b1; b++) {
+                            const float * p = part(b, b == b0);
+                            const float m2 = __ldcg(p + D * 128);
+                            const float w = m2 == m ? 1.0f : exp2_fast(m2 - m);
+                            l = fmaf(__ldcg(p + (D + 1) * 128), w, l);
+#pragma unroll
+                            for (int d = 0; d < D; d++) {
+                                o[d] = fmaf(__ldcg(p + d * 128), w, o[d]);
+                            }
+                        }
+                    }
+                }
+                if (write && live) {
+                    const float inv = l > 0.0f || isnan(l) ? a.v_scale / l : 0.0f; // no visible key: zeros
+                    float * out = a.out + (size_t)(u.r.row0 + tok) * a.out_stride + (size_t)head * D;
+                    if (a.vec) {
+#pragma unroll
+                        for (int d = 0; d < D; d += 4) {
+                            *reinterpret_cast<float4 *>(out + d) = make_float4(o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
+                        }
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < D; d++) {
+                            out[d] = o[d] * inv;
+                        }
+                    }
+                }
+            }
+            tile_n += (uint32_t)n;
+            left -= n;
+            at += n;
+            if (left <= 0) {
+                break;
+            }
+            advance(x, left, u);
+        }
+    }
+};
+
+template <int T, int D> __global__ void __launch_bounds__(kPrThreads, 1) attn_prompt_kernel(const __grid_constant__ AttnDev a) {
+    extern __shared__ uint8_t smem_raw[];
+    using P = Prompt<T, D>;
+    const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t * gen = smem_raw + (base - raw);
+    constexpr uint32_t HDR = (4 + P::SLOTS) * P::TILE;
+    const uint32_t hdr = base + HDR;
+    // header: q_full[2] @0, s_full[2] @16, p_full[2] @32, drain @48, kv_full[6] @64, kv_empty[6] @128, sums @192,
+    // seen groups of eight tiles @256, last[2] @320, tensor memory address @328, fail @332, found share @336
+    P p{a, base, hdr, 0, reinterpret_cast<volatile int *>(gen + HDR + 332), {hdr, hdr + 16, hdr + 32, hdr + 64, hdr + 128, hdr + 48}};
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (tid == 0) {
+        for (int t = 0; t < 2; t++) {
+            mbar_init(p.bars.q_full + 8 * t, 128);
+            mbar_init(p.bars.s_full + 8 * t, 1);
+            mbar_init(p.bars.p_full + 8 * t, 128);
+        }
+        for (int s = 0; s < P::SLOTS; s++) {
+            mbar_init(p.bars.kv_full + 8 * s, kPrProducers);
+            mbar_init(p.bars.kv_empty + 8 * s, 1);
+        }
+        mbar_init(p.bars.drain, 1);
+        *p.fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        tmem_alloc(hdr + 328, 512);
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    // ---- the CTA's share of the list: units by (sequence, row block, KV head).  The first blocks of the sequences
+    // go through shared memory (the tiles' space, not yet in use), then the threads look at a (sequence, row block) each.
+    int * first_block = reinterpret_cast<int *>(gen); // [n_seq + 1]
+    volatile int * s_sum = reinterpret_cast<volatile int *>(gen + HDR + 192); // one a warp
+    auto block_scan = [&](int v, int & before) { // sum over the threads below; returns the block's sum
+        int y = v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int z = __shfl_up_sync(~0u, y, d);
+            y += lane >= d ? z : 0;
+        }
+        __syncthreads();
+        if (lane == 31) {
+            s_sum[warp] = y;
+        }
+        __syncthreads();
+        int all = 0, mine = 0;
+#pragma unroll
+        for (int w = 0; w < kPrThreads / 32; w++) {
+            mine += w < warp ? s_sum[w] : 0;
+            all += s_sum[w];
+        }
+        before = mine + y - v;
+        return all;
+    };
+    int n_pairs = 0, before;
+    for (int s0 = 0; s0 < a.b.n_seq; s0 += kPrThreads) {
+        const int s = s0 + tid;
+        const int v = s < a.b.n_seq ? (seq_rows(a.b, a.kv.page_shift, s).n_run * a.group + kPrRows - 1) / kPrRows : 0;
+        const int all = block_scan(v, before);
+        if (s < a.b.n_seq) {
+            first_block[s] = n_pairs + before;
+        }
+        n_pairs += all;
+    }
+    __syncthreads();
+    auto find = [&](int pair, int & s, int & rb) { // the last sequence whose first block is not behind the pair
+        int lo = 0, hi = a.b.n_seq;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (first_block[mid] <= pair) {
+                lo = mid;
+            } else {
+                hi = mid;
+            }
+        }
+        s = lo;
+        rb = pair - first_block[lo];
+    };
+    long long total = 0;
+    for (int p0 = 0; p0 < n_pairs; p0 += kPrThreads) {
+        int v = 0, s, rb;
+        if (p0 + tid < n_pairs) {
+            find(p0 + tid, s, rb);
+            v = p.unit(s, rb).k.count;
+        }
+        total += (long long)block_scan(v, before) * a.kv.n_kv;
+    }
+    const long long want = (total + a.min_tiles - 1) / a.min_tiles;
+    const long long nw = max(1LL, want < gridDim.x ? want : gridDim.x);
+    const long long each = total / nw, more = total - each * nw;
+    const long long c0 = blockIdx.x * each + min((long long)blockIdx.x, more);
+    const long long c1 = c0 + each + (blockIdx.x < more ? 1 : 0);
+    const bool work = blockIdx.x < nw && c1 > c0;
+    PromptSeg seg = {};
+    volatile int * found = reinterpret_cast<volatile int *>(gen + HDR + 336); // s, rb, head, tile
+    if (work) {
+        long long run = 0;
+        for (int p0 = 0; p0 < n_pairs; p0 += kPrThreads) {
+            int v = 0, s = 0, rb = 0;
+            if (p0 + tid < n_pairs) {
+                find(p0 + tid, s, rb);
+                v = p.unit(s, rb).k.count;
+            }
+            const int all = block_scan(v, before);
+            const long long b = run + (long long)before * a.kv.n_kv;
+            if (v > 0 && c0 >= b && c0 < b + (long long)v * a.kv.n_kv) {
+                const int in = (int)(c0 - b);
+                found[0] = s;
+                found[1] = rb;
+                found[2] = in / v;
+                found[3] = in % v;
+            }
+            run += (long long)all * a.kv.n_kv;
+            if (run > c0) {
+                break;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    p.tmem = *reinterpret_cast<volatile uint32_t *>(gen + HDR + 328);
+    if (work) {
+        seg.s = found[0];
+        seg.rb = found[1];
+        seg.h = found[2];
+        seg.t_begin = found[3];
+        const PromptUnit u = p.unit(seg.s, seg.rb);
+        const long long left = c1 - c0;
+        const int here = u.k.count - seg.t_begin;
+        seg.t_end = seg.t_begin + (int)(left < here ? left : here);
+        if (warp < 8) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+            p.softmax(seg, u, left, c0, each, more);
+        } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+            if (warp > 8) {
+                p.produce(seg, u, left);
+            } else if (lane == 0) {
+                p.multiply(seg, u, left);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tmem_dealloc(p.tmem, 512);
+    }
+}
+
+template <int T, int D> static cudaError_t launch_t(cudaStream_t s, const AttnDev & a) {
+    const cudaError_t e = ensure_dynamic_smem((const void *)attn_prompt_kernel<T, D>, pr_smem(D));
+    if (e != cudaSuccess) {
+        return e;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kSMs);
+    cfg.blockDim = dim3(kPrThreads);
+    cfg.dynamicSmemBytes = pr_smem(D);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attn_prompt_kernel<T, D>, a);
+}
+
+size_t attn_prompt_units(int n_head, int n_kv, int n_seq, int max_q) { // counters: two tiles a unit
+    return (size_t)n_seq * n_kv * (((size_t)max_q * (n_head / n_kv) + kPrRows - 1) / kPrRows) * 2;
+}
+size_t attn_prompt_part_bytes(int head_dim) { return (size_t)kSMs * 4 * pr_part_floats(head_dim) * sizeof(float); }
+
+cudaError_t launch_attn_prompt(cudaStream_t s, AttnDev a) {
+    a.row_blocks = (int)(((long long)a.b.max_q * a.group + kPrRows - 1) / kPrRows);
+    a.min_tiles = 2;
+    a.vec = !((uintptr_t)a.q & 15) && !((uintptr_t)a.out & 15) && !(a.q_stride & 3) && !(a.out_stride & 3);
+    switch (a.kv.type) {
+    case kF16: return a.kv.head_dim == 64 ? launch_t<kF16, 64>(s, a) : launch_t<kF16, 128>(s, a);
+    case kBF16: return a.kv.head_dim == 64 ? launch_t<kBF16, 64>(s, a) : launch_t<kBF16, 128>(s, a);
+    default: return a.kv.head_dim == 64 ? launch_t<kE4M3, 64>(s, a) : launch_t<kE4M3, 128>(s, a);
+    }
+}
+
+cudaError_t read_attn_prompt_status(int * status, bool clear) {
+    cudaError_t e = cudaMemcpyFromSymbol(status, g_attn_prompt_status, sizeof(int));
+    if (e == cudaSuccess && clear && *status != 0) {
+        const int zero = 0;
+        e = cudaMemcpyToSymbol(g_attn_prompt_status, &zero, sizeof(int));
+    }
+    return e;
+}
+
+} // namespace b200q

@@ -716,6 +716,12 @@ int b200q_device_status(int * status, int clear) {
     page = page ? page : word;
     B200Q_CUDA_OK(read_pages_status(&word, clear != 0));
     page = page ? page : word;
+    B200Q_CUDA_OK(read_attn_prompt_status(&word, clear != 0));
+    if (word == B200Q_ETIMEOUT) {
+        *status = *status ? *status : word;
+    } else {
+        page = page ? page : word;
+    }
     if (*status != 0) {
         set_error("a bounded device-side wait ran out (status %d)", *status);
     } else if (page != 0) {

@@ -59,6 +59,10 @@ static int check_batch(const char * who, const b200q_kv_batch * b, BatchDev & d)
                   b->table_stride);
         return B200Q_EINVAL;
     }
+    if (b->n_seq > kMaxSeqs) {
+        set_error("%s: a step holds up to %d sequences (got %d)", who, kMaxSeqs, b->n_seq);
+        return B200Q_EUNSUPPORTED;
+    }
     d.page_table = b->page_table;
     d.q_start = b->q_start;
     d.kv_len = b->kv_len;
@@ -91,6 +95,11 @@ static bool rows_overlap(const float * a, int a_stride, int a_n, const float * b
     return true;
 }
 
+// arrival counters of a call
+static size_t attn_units(int n_head, int n_kv, int n_seq, int max_q) {
+    return (long long)max_q * (n_head / n_kv) <= kDecodeRows ? attn_decode_units(n_head, n_kv, n_seq, max_q)
+                                                             : attn_prompt_units(n_head, n_kv, n_seq, max_q);
+}
 static size_t counter_bytes(size_t units) { return (units * sizeof(uint32_t) + 255) / 256 * 256; }
 
 } // namespace b200q
@@ -174,7 +183,9 @@ size_t b200q_attn_scratch_bytes(int n_head, int n_kv, int head_dim, int n_seq, i
         return 0;
     }
     const int mq = max_q < n_tok ? max_q : (n_tok > 0 ? n_tok : 1);
-    return counter_bytes(attn_decode_units(n_head, n_kv, n_seq, mq)) + attn_decode_part_bytes(n_head, n_kv, head_dim, mq);
+    const size_t parts = (long long)mq * (n_head / n_kv) <= kDecodeRows ? attn_decode_part_bytes(n_head, n_kv, head_dim, mq)
+                                                                        : attn_prompt_part_bytes(head_dim);
+    return counter_bytes(attn_units(n_head, n_kv, n_seq, mq)) + parts;
 }
 
 int b200q_attn(void * stream, const float * q, int q_stride, int n_head, const b200q_kv_cache * cache,
@@ -214,7 +225,7 @@ int b200q_attn(void * stream, const float * q, int q_stride, int n_head, const b
         a.window = opts->window;
         a.n_sink = opts->window ? opts->n_sink : 0;
     }
-    const size_t units = attn_decode_units(n_head, a.kv.n_kv, a.b.n_seq, a.b.max_q);
+    const size_t units = attn_units(n_head, a.kv.n_kv, a.b.n_seq, a.b.max_q);
     const size_t need = b200q_attn_scratch_bytes(n_head, a.kv.n_kv, D, a.b.n_seq, a.b.n_tok, a.b.max_q);
     if (!scratch || !aligned(scratch, 16) || scratch_bytes < need) {
         set_error("%s: scratch must be 16-byte aligned and hold %zu bytes (got %zu)", who, need, scratch_bytes);
@@ -233,7 +244,11 @@ int b200q_attn(void * stream, const float * q, int q_stride, int n_head, const b
     a.v_scale = a.kv.v_scale;
     a.counters = static_cast<uint32_t *>(scratch);
     a.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + counter_bytes(units));
-    B200Q_CUDA_OK(launch_attn_decode((cudaStream_t)stream, a));
+    if ((long long)a.b.max_q * a.group <= kDecodeRows) {
+        B200Q_CUDA_OK(launch_attn_decode((cudaStream_t)stream, a));
+    } else {
+        B200Q_CUDA_OK(launch_attn_prompt((cudaStream_t)stream, a));
+    }
     return B200Q_OK;
 }
 

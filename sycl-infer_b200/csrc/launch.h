@@ -88,10 +88,11 @@ cudaError_t launch_probe_read(cudaStream_t s, const void * buf, size_t bytes, ui
 cudaError_t launch_probe_i8_mma(cudaStream_t s, int iters, uint32_t * sink);
 cudaError_t read_probe_status(int * status, bool clear);
 
-// status words of the attention-side kernels (rope_append.cu, attn_decode.cu, kv_pages.cu): a bad page id
+// status words of the attention-side kernels (rope_append.cu, attn_decode.cu, attn_prompt.cu, kv_pages.cu): a bad page id
 cudaError_t read_append_status(int * status, bool clear);
 cudaError_t read_attn_status(int * status, bool clear);
 cudaError_t read_pages_status(int * status, bool clear);
+cudaError_t read_attn_prompt_status(int * status, bool clear); // also: a bounded wait ran out
 
 cudaError_t launch_peer_barrier(cudaStream_t s, uint32_t * const * flags, int world, int rank, uint32_t seq);
 cudaError_t read_peer_status(int * status, bool clear);
