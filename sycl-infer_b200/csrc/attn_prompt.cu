@@ -49,7 +49,7 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, u
                  "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
                  : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint64_t (&v)[16]) { // 32 columns, in pairs
     uint32_t * u = reinterpret_cast<uint32_t *>(v);
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
                  "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -67,6 +67,30 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&u)[16
                  : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// pairs of fp32 in one register pair
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float first2(uint64_t a) { return __uint_as_float((uint32_t)a); }
+__device__ __forceinline__ float second2(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 
 // Shared-memory operand descriptor, 128-byte swizzle: rows of 128 bytes in atoms of eight, `lbo` and `sbo` the byte
 // distances between atoms (see the uses).
@@ -112,9 +136,20 @@ struct PromptUnit {
     int rows;   // rows of this block, at most kPrRows
     int row0;   // first row among the sequence's (token, head) rows
 };
+// A CTA's share of the list is measured in tiles plus kPrUnitCost a unit (its q, its join, its rows out): tile i of a unit
+// that starts at position `pos` of the list lies at pos + kPrUnitCost + i.
+constexpr int kPrUnitCost = 1;
 struct PromptSeg {
     int s, h, rb;
     int t_begin, t_end;
+    long long pos;
+};
+// CTA b's share starts at b * each + min(b, more).
+struct PromptShare {
+    long long each, more, end;
+    __device__ __forceinline__ int owner(long long x) const { // the CTA whose share holds position x
+        return (int)(x < more * (each + 1) ? x / (each + 1) : more + (x - more * (each + 1)) / each);
+    }
 };
 
 struct PromptBars {
@@ -132,6 +167,7 @@ template <int T, int D> struct Prompt {
     uint32_t tmem;
     volatile int * fail;
     PromptBars bars;
+    PromptShare share;
 
     __device__ __forceinline__ uint32_t q_addr(int tile, int part) const { return base + (tile * 2 + part) * TILE; }
     __device__ __forceinline__ uint32_t slot_addr(int slot) const { return base + (4 + slot) * TILE; }
@@ -158,8 +194,12 @@ template <int T, int D> struct Prompt {
         u.k = key_tiles(pos0, min(u.r.n, max(pos1 + 1, 0)), kPrKeys, a.window, a.n_sink);
         return u;
     }
-    // to the next unit of the share, `left` tiles still to come (> 0)
-    __device__ __forceinline__ void advance(PromptSeg & x, long long left, PromptUnit & u) const {
+    // to the next unit of the share; false: there is none
+    __device__ __forceinline__ bool advance(PromptSeg & x, PromptUnit & u) const {
+        x.pos += u.k.count + kPrUnitCost;
+        if (x.pos + kPrUnitCost >= share.end) {
+            return false;
+        }
         // heads innermost: neighbouring CTAs read neighbouring heads of the same pages
         if (++x.h == a.kv.n_kv) {
             x.h = 0;
@@ -174,11 +214,12 @@ template <int T, int D> struct Prompt {
             }
         }
         x.t_begin = 0;
-        x.t_end = (int)(left < u.k.count ? left : u.k.count);
+        x.t_end = (int)min((long long)u.k.count, share.end - x.pos - kPrUnitCost);
+        return true;
     }
 
     // ---- warp 8, one thread: the products
-    __device__ void multiply(PromptSeg x, PromptUnit u, long long left) const {
+    __device__ void multiply(PromptSeg x, PromptUnit u) const {
         const uint32_t id_qk = idesc_f16(BF, false, kPrKeys), id_pv = idesc_f16(BF, true, D);
         uint32_t p_par = 0, q_par = 0, item = 0; // a bit a tile: the phase that is waited for
         auto s_cols = [&](int t) { return tmem + (uint32_t)t * 128; };
@@ -237,6 +278,9 @@ template <int T, int D> struct Prompt {
                     }
                     tc_fence_after();
                     values(t, iv % SLOTS);
+                    if (t == tiles - 1) {
+                        release(iv); // before the scores: the next tile's keys take this place
+                    }
                     if (j + 1 < n) {
                         if (t == 0) {
                             full(ik);
@@ -246,24 +290,21 @@ template <int T, int D> struct Prompt {
                     }
                     mma_commit(bars.s_full + 8 * t);
                 }
-                release(iv);
                 if (j + 1 < n) {
                     release(ik);
                 }
             }
             item += 2 * n;
-            left -= n;
-            if (left <= 0) {
+            if (!advance(x, u)) {
                 break;
             }
-            advance(x, left, u);
         }
         mma_commit(bars.drain); // tensor memory is given back only when every product is done
         mbar_wait(bars.drain, 0, &g_attn_prompt_status);
     }
 
     // ---- warps 9-11: K and V into shared memory
-    __device__ void produce(PromptSeg x, PromptUnit u, long long left) const {
+    __device__ void produce(PromptSeg x, PromptUnit u) const {
         constexpr int EB = KvElem<T>::BYTES, ROWB = D * EB;
         constexpr int PIECES = kPrKeys * ROWB / 512;    // runs of 32 chunks of 16 bytes: one a warp
         constexpr int PER_GROUP = 16 * ROWB / 512;      // of a group of 16 keys
@@ -379,147 +420,174 @@ template <int T, int D> struct Prompt {
                     }
                 }
             }
-            left -= x.t_end - x.t_begin;
-            if (left <= 0) {
+            if (!advance(x, u)) {
                 break;
             }
-            advance(x, left, u);
         }
         flush(true);
     }
 
     // ---- warps 0-3 and 4-7: softmax, a thread a row of its tile
-    __device__ void softmax(PromptSeg x, PromptUnit u, long long left, long long at, long long each, long long more) const {
-        const int tid = threadIdx.x & 127, t = (int)(threadIdx.x >> 7);
-        const uint32_t lanes = (uint32_t)(32 * ((threadIdx.x >> 5) & 3)) << 16;
+    __device__ void softmax(PromptSeg x, PromptUnit u) const {
+        const int tid = threadIdx.x & 127, t = (int)(threadIdx.x >> 7), lane = threadIdx.x & 31, warp_row = tid & ~31;
+        const uint32_t lanes = (uint32_t)warp_row << 16;
         const uint32_t s_cols = tmem + lanes + (uint32_t)t * 128, o_cols = tmem + lanes + 256 + (uint32_t)t * 128;
         const volatile int * meta = reinterpret_cast<const volatile int *>(__cvta_shared_to_generic(hdr + 256));
         volatile int * last = reinterpret_cast<volatile int *>(__cvta_shared_to_generic(hdr + 320)) + t;
-        uint32_t s_n = 0, tile_n = 0;
+        uint32_t s_par = 0, tile_n = 0;
+        constexpr int RPL = 128 / D; // rows that one coalesced access of the warp covers (32 lanes of four values)
         for (;;) {
             const int n = x.t_end - x.t_begin;
             const bool mine = t == 0 || u.rows > 128; // the second tile may be empty
             if (mine) {
-                const int r = u.row0 + t * 128 + tid, r_end = u.row0 + u.rows;
+                const int r0 = u.row0 + t * 128, r = r0 + tid, r_end = u.row0 + u.rows;
                 const bool live = r < r_end;
                 const int first = u.r.n - u.r.n_row;
                 const int tok = live ? r / a.group : 0, head = x.h * a.group + (live ? r - tok * a.group : 0);
                 const int pos = live ? first + tok : -1;
-                const int pos_min = first + (u.row0 + t * 128) / a.group;
-                const int pos_max = first + (min(u.row0 + t * 128 + 127, r_end - 1)) / a.group;
-                const float * q = a.q + (size_t)(u.r.row0 + tok) * a.q_stride + (size_t)head * D;
-                // q in two parts to shared memory
+                const int pos_min = first + r0 / a.group, pos_max = first + min(r0 + 127, r_end - 1) / a.group;
+                const uint32_t live_rows = __ballot_sync(~0u, live); // of the warp's 32
+                // q in two parts to shared memory, rows read whole by the warp
                 float cq = a.scale_log2;
-                float up = 1.0f;
-                auto q4 = [&](int d) {
-                    if (!live) {
-                        return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const long long q_at = (long long)(u.r.row0 + tok) * a.q_stride + (long long)head * D;
+                const int d = lane % (32 / RPL) * 4;
+#pragma unroll 1
+                for (int i0 = 0; i0 < 32; i0 += 8 * RPL) {
+                    float4 v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int row = i0 + i * RPL + lane / (32 / RPL);
+                        const float * q = a.q + __shfl_sync(~0u, q_at, row) + d;
+                        v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if ((live_rows >> row) & 1) {
+                            if (a.vec) {
+                                v[i] = __ldg(reinterpret_cast<const float4 *>(q));
+                            } else {
+                                v[i] = make_float4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
+                            }
+                        }
                     }
-                    if (a.vec) {
-                        return __ldg(reinterpret_cast<const float4 *>(q + d));
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int row = i0 + i * RPL + lane / (32 / RPL);
+                        if constexpr (!BF) {
+                            float top = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+#pragma unroll
+                            for (int w = 16 / RPL; w > 0; w >>= 1) {
+                                top = fmaxf(top, __shfl_xor_sync(~0u, top, w));
+                            }
+                            const int e = pow2_to_top(top);
+                            const float up = exp2_int(e);
+                            v[i] = make_float4(v[i].x * up, v[i].y * up, v[i].z * up, v[i].w * up);
+                            // the thread of the row takes the factor back out of the scores
+#pragma unroll
+                            for (int k = 0; k < RPL; k++) {
+                                const int back = __shfl_sync(~0u, e, k * (32 / RPL));
+                                cq *= lane == i0 + i * RPL + k ? exp2_int(-back) : 1.0f;
+                            }
+                        }
+                        uint32_t p0[2], p1[2];
+                        split_pair<T>(v[i].x, v[i].y, p0);
+                        split_pair<T>(v[i].z, v[i].w, p1);
+                        const uint32_t to = sw128_off(warp_row + row, d / 8) + (uint32_t)(d & 4) * 2;
+                        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(q_addr(t, 0) + to), "r"(p0[0]), "r"(p1[0]) : "memory");
+                        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(q_addr(t, 1) + to), "r"(p0[1]), "r"(p1[1]) : "memory");
                     }
-                    return make_float4(__ldg(q + d), __ldg(q + d + 1), __ldg(q + d + 2), __ldg(q + d + 3));
-                };
-                if constexpr (!BF) {
-                    float top = 0.0f;
-#pragma unroll 8
-                    for (int d = 0; d < D; d += 4) {
-                        const float4 v = q4(d);
-                        top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-                    }
-                    const int e = pow2_to_top(top);
-                    up = exp2_int(e);
-                    cq *= exp2_int(-e);
-                }
-#pragma unroll 4
-                for (int c = 0; c < D / 8; c++) {
-                    const float4 v = q4(c * 8), w = q4(c * 8 + 4);
-                    uint32_t p0[2], p1[2], p2[2], p3[2];
-                    split_pair<T>(v.x * up, v.y * up, p0);
-                    split_pair<T>(v.z * up, v.w * up, p1);
-                    split_pair<T>(w.x * up, w.y * up, p2);
-                    split_pair<T>(w.z * up, w.w * up, p3);
-                    sts128(q_addr(t, 0) + sw128_off(tid, c), p0[0], p1[0], p2[0], p3[0]);
-                    sts128(q_addr(t, 1) + sw128_off(tid, c), p0[1], p1[1], p2[1], p3[1]);
                 }
                 fence_proxy_async();
                 mbar_arrive(bars.q_full + 8 * t);
 
-                float o[D];
+                uint64_t o[D / 2]; // pairs of fp32
 #pragma unroll
-                for (int d = 0; d < D; d++) {
-                    o[d] = 0.0f;
+                for (int i = 0; i < D / 2; i++) {
+                    o[i] = 0;
                 }
                 float m = -INFINITY, l = 0.0f, f = 1.0f;
                 const int low = a.window ? pos - a.window + 1 : 0;
                 auto add_o = [&]() { // o = o f + the tile's p v
+                    const uint64_t ff = pair2(f, f);
 #pragma unroll
                     for (int c = 0; c < D / 32; c++) {
-                        float v[32];
+                        uint64_t v[16];
                         tmem_ld32(o_cols + 32 * c, v);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            o[32 * c + i] = fmaf(o[32 * c + i], f, v[i]);
+                        for (int i = 0; i < 16; i++) {
+                            o[16 * c + i] = fma2(o[16 * c + i], ff, v[i]);
                         }
                     }
                 };
-                for (int j = 0; j < n; j++) {
-                    wait(bars.s_full + 8 * t, s_n & 1);
-                    s_n++;
+                auto next_s = [&]() {
+                    wait(bars.s_full + 8 * t, s_par);
+                    s_par ^= 1;
                     __syncwarp();
                     tc_fence_after();
+                };
+                for (int j = 0; j < n; j++) {
+                    next_s();
                     const int key0 = key_tile(u.k, x.t_begin + j) * kPrKeys;
                     const uint32_t valid = (uint32_t)meta[(tile_n + j) & 7];
                     const bool whole = valid == 0xFFu && key0 + kPrKeys - 1 <= pos_min &&
                                        (a.window == 0 || key0 > pos_max - a.window || key0 + kPrKeys <= a.n_sink);
-                    const int c_hi = pos - key0, c_lo = low - key0, c_sink = a.n_sink - key0;
-                    auto load = [&](int c, float (&v)[32]) {
-                        tmem_ld32(s_cols + 32 * c, v);
+                    // columns that the row sees, of 32 from column c on
+                    auto seen = [&](int c) {
+                        auto below = [](int k) { return k >= 32 ? ~0u : (k <= 0 ? 0u : (1u << k) - 1u); }; // bits 0 .. k-1
+                        const uint32_t groups = ((valid >> (c / 16)) & 1 ? 0xFFFFu : 0u) | ((valid >> (c / 16 + 1)) & 1 ? 0xFFFF0000u : 0u);
+                        return groups & below(pos + 1 - key0 - c) & (~below(low - key0 - c) | below(a.n_sink - key0 - c));
+                    };
+                    auto load = [&](int c, uint64_t (&v)[16]) {
+                        tmem_ld32(s_cols + c, v);
                         tmem_ld_wait();
                         if (!whole) {
+                            const uint32_t bits = seen(c);
 #pragma unroll
-                            for (int i = 0; i < 32; i++) {
-                                const int col = 32 * c + i;
-                                const bool seen = col <= c_hi && (col >= c_lo || col < c_sink) && ((valid >> (2 * c + i / 16)) & 1);
-                                v[i] = seen ? v[i] : -INFINITY;
+                            for (int i = 0; i < 16; i++) {
+                                v[i] = pair2((bits >> (2 * i)) & 1 ? first2(v[i]) : -INFINITY,
+                                             (bits >> (2 * i + 1)) & 1 ? second2(v[i]) : -INFINITY);
                             }
                         }
                     };
                     float top = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        float v[32];
+#pragma unroll 1
+                    for (int c = 0; c < kPrKeys; c += 32) {
+                        uint64_t v[16];
                         load(c, v);
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            top = fmaxf(top, fmaxf(v[i], v[i + 1]));
+                        for (int i = 0; i < 16; i++) {
+                            top = fmaxf(top, fmaxf(first2(v[i]), second2(v[i])));
                         }
                     }
                     const float mn = fmaxf(m, top * cq);
                     const float f_new = m == mn ? 1.0f : exp2_fast(m - mn);
                     const float off = BIAS - (mn == -INFINITY ? 0.0f : mn);
                     m = mn;
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        float v[32];
+                    uint64_t sum = 0, sum1 = 0;
+                    const uint64_t cc = pair2(cq, cq), oo = pair2(off, off);
+#pragma unroll 1
+                    for (int c = 0; c < kPrKeys; c += 32) {
+                        uint64_t v[16];
                         load(c, v);
                         uint32_t hi[16], lo[16];
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float p0 = exp2_fast(fmaf(v[i], cq, off)), p1 = exp2_fast(fmaf(v[i + 1], cq, off));
-                            sum[i & 2] += p0;
-                            sum[(i & 2) + 1] += p1;
+                        for (int i = 0; i < 16; i++) {
+                            const uint64_t e = fma2(v[i], cc, oo);
+                            const float p0 = exp2_fast(first2(e)), p1 = exp2_fast(second2(e));
+                            const uint64_t pp = pair2(p0, p1);
+                            if (i & 1) {
+                                sum1 = add2(sum1, pp);
+                            } else {
+                                sum = add2(sum, pp);
+                            }
                             uint32_t part[2];
                             split_pair<T>(p0, p1, part);
-                            hi[i / 2] = part[0];
-                            lo[i / 2] = part[1];
+                            hi[i] = part[0];
+                            lo[i] = part[1];
                         }
-                        tmem_st16(s_cols + 32 * c, hi); // over the 32 columns of s that were just read
-                        tmem_st16(s_cols + 32 * c + 16, lo);
+                        tmem_st16(s_cols + c, hi); // over the 32 columns of s that were just read
+                        tmem_st16(s_cols + c + 16, lo);
                     }
-                    l = fmaf(l, f_new, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                    sum = add2(sum, sum1);
+                    l = fmaf(l, f_new, first2(sum) + second2(sum));
                     if (j > 0) {
                         add_o(); // of the tile before: complete, its commit came before this tile's s
                     }
@@ -528,32 +596,29 @@ template <int T, int D> struct Prompt {
                     tc_fence_before();
                     mbar_arrive(bars.p_full + 8 * t);
                 }
-                wait(bars.s_full + 8 * t, s_n & 1);
-                s_n++;
-                __syncwarp();
-                tc_fence_after();
+                next_s();
                 add_o();
                 tc_fence_before();
 
                 bool write = true;
-                if (n != u.k.count) {
-                    // the unit spans CTAs: its tiles are [u0, u0 + count) of the list
-                    const long long u0 = at - x.t_begin;
-                    auto owner = [&](long long y) { // the CTA whose share holds tile y
-                        return (int)(y < more * (each + 1) ? y / (each + 1) : more + (y - more * (each + 1)) / each);
-                    };
-                    const int b0 = owner(u0), b1 = owner(u0 + u.k.count - 1);
+                if (n != u.k.count) { // the unit spans CTAs
+                    const int b0 = share.owner(x.pos + kPrUnitCost), b1 = share.owner(x.pos + kPrUnitCost + u.k.count - 1);
+                    // four columns of a thread lie together, a warp's 512 bytes side by side
                     auto part = [&](int b, bool second) {
-                        return a.parts + ((size_t)(b * 2 + (second ? 1 : 0)) * 2 + t) * pr_part_floats(D) + tid;
+                        return a.parts + ((size_t)(b * 2 + (second ? 1 : 0)) * 2 + t) * pr_part_floats(D) + tid * 4;
+                    };
+                    auto stats = [&](int b, bool second) {
+                        return a.parts + ((size_t)(b * 2 + (second ? 1 : 0)) * 2 + t) * pr_part_floats(D) + D * 128 + tid;
                     };
                     // of a CTA's two places the second holds the unit that starts in its share and runs on behind it
-                    float * mine_p = part((int)blockIdx.x, x.t_begin == 0);
+                    const bool second = x.t_begin == 0;
+                    float * to = part((int)blockIdx.x, second), * st = stats((int)blockIdx.x, second);
 #pragma unroll
-                    for (int d = 0; d < D; d++) {
-                        mine_p[d * 128] = o[d];
+                    for (int i = 0; i < D / 4; i++) {
+                        *reinterpret_cast<float4 *>(to + i * 512) = make_float4(first2(o[2 * i]), second2(o[2 * i]), first2(o[2 * i + 1]), second2(o[2 * i + 1]));
                     }
-                    mine_p[D * 128] = m;
-                    mine_p[(D + 1) * 128] = l;
+                    st[0] = m;
+                    st[128] = l;
                     __threadfence();
                     tile_sync(t);
                     if (tid == 0) {
@@ -570,48 +635,63 @@ template <int T, int D> struct Prompt {
                     if (write) {
                         m = -INFINITY;
                         for (int b = b0; b <= b1; b++) {
-                            m = fmaxf(m, __ldcg(part(b, b == b0) + D * 128));
+                            m = fmaxf(m, __ldcg(stats(b, b == b0)));
                         }
                         l = 0.0f;
 #pragma unroll
-                        for (int d = 0; d < D; d++) {
-                            o[d] = 0.0f;
+                        for (int i = 0; i < D / 2; i++) {
+                            o[i] = 0;
                         }
                         for (int b = b0; b <= b1; b++) {
-                            const float * p = part(b, b == b0);
-                            const float m2 = __ldcg(p + D * 128);
+                            const float * p = part(b, b == b0), * s2 = stats(b, b == b0);
+                            const float m2 = __ldcg(s2);
                             const float w = m2 == m ? 1.0f : exp2_fast(m2 - m);
-                            l = fmaf(__ldcg(p + (D + 1) * 128), w, l);
+                            const uint64_t ww = pair2(w, w);
+                            l = fmaf(__ldcg(s2 + 128), w, l);
 #pragma unroll
-                            for (int d = 0; d < D; d++) {
-                                o[d] = fmaf(__ldcg(p + d * 128), w, o[d]);
+                            for (int i = 0; i < D / 4; i++) {
+                                const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + i * 512));
+                                o[2 * i] = fma2(pair2(v.x, v.y), ww, o[2 * i]);
+                                o[2 * i + 1] = fma2(pair2(v.z, v.w), ww, o[2 * i + 1]);
                             }
                         }
                     }
                 }
-                if (write && live) {
+                if (write) {
+                    // through the tile's q space, whose products are done, so that rows leave whole; the warp's own 32 rows
                     const float inv = l > 0.0f || isnan(l) ? a.v_scale / l : 0.0f; // no visible key: zeros
-                    float * out = a.out + (size_t)(u.r.row0 + tok) * a.out_stride + (size_t)head * D;
-                    if (a.vec) {
+                    const uint64_t ii = pair2(inv, inv);
+                    const uint32_t stage = q_addr(t, 0) + (uint32_t)warp_row * D * 4;
 #pragma unroll
-                        for (int d = 0; d < D; d += 4) {
-                            *reinterpret_cast<float4 *>(out + d) = make_float4(o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
-                        }
-                    } else {
-#pragma unroll
-                        for (int d = 0; d < D; d++) {
-                            out[d] = o[d] * inv;
+                    for (int i = 0; i < D / 4; i++) {
+                        const uint64_t lo2 = mul2(o[2 * i], ii), hi2 = mul2(o[2 * i + 1], ii);
+                        sts128(stage + (uint32_t)(lane * D * 4 + ((i ^ (lane & 7)) << 4)), (uint32_t)lo2, (uint32_t)(lo2 >> 32), (uint32_t)hi2,
+                               (uint32_t)(hi2 >> 32));
+                    }
+                    __syncwarp();
+                    const long long out_at = (long long)(u.r.row0 + tok) * a.out_stride + (long long)head * D;
+#pragma unroll 8
+                    for (int i = 0; i < 32; i += RPL) {
+                        const int row = i + lane / (32 / RPL);
+                        float v[4];
+                        const uint32_t from = stage + (uint32_t)(row * D * 4 + (((d / 4) ^ (row & 7)) << 4));
+                        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(from) : "memory");
+                        float * out = a.out + __shfl_sync(~0u, out_at, row) + d;
+                        if ((live_rows >> row) & 1) {
+                            if (a.vec) {
+                                *reinterpret_cast<float4 *>(out) = make_float4(v[0], v[1], v[2], v[3]);
+                            } else {
+                                out[0] = v[0], out[1] = v[1], out[2] = v[2], out[3] = v[3];
+                            }
                         }
                     }
+                    __syncwarp(); // the space takes the next unit's q
                 }
             }
             tile_n += (uint32_t)n;
-            left -= n;
-            at += n;
-            if (left <= 0) {
+            if (!advance(x, u)) {
                 break;
             }
-            advance(x, left, u);
         }
     }
 };
@@ -625,7 +705,7 @@ template <int T, int D> __global__ void __launch_bounds__(kPrThreads, 1) attn_pr
     const uint32_t hdr = base + HDR;
     // header: q_full[2] @0, s_full[2] @16, p_full[2] @32, drain @48, kv_full[6] @64, kv_empty[6] @128, sums @192,
     // seen groups of eight tiles @256, last[2] @320, tensor memory address @328, fail @332, found share @336
-    P p{a, base, hdr, 0, reinterpret_cast<volatile int *>(gen + HDR + 332), {hdr, hdr + 16, hdr + 32, hdr + 64, hdr + 128, hdr + 48}};
+    P p{a, base, hdr, 0, reinterpret_cast<volatile int *>(gen + HDR + 332), {hdr, hdr + 16, hdr + 32, hdr + 64, hdr + 128, hdr + 48}, {0, 0, 0}};
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 0) {
@@ -697,31 +777,38 @@ template <int T, int D> __global__ void __launch_bounds__(kPrThreads, 1) attn_pr
         rb = pair - first_block[lo];
     };
     long long total = 0;
-    for (int p0 = 0; p0 < n_pairs; p0 += kPrThreads) {
-        int v = 0, s, rb;
-        if (p0 + tid < n_pairs) {
-            find(p0 + tid, s, rb);
-            v = p.unit(s, rb).k.count;
+    auto cost = [&](int pair, int & s, int & rb) { // of the pair's unit of one head
+        if (pair >= n_pairs) {
+            return 0;
         }
-        total += (long long)block_scan(v, before) * a.kv.n_kv;
+        find(pair, s, rb);
+        return p.unit(s, rb).k.count + kPrUnitCost;
+    };
+    int s_first = 0, rb_first = 0, before_first = 0;
+    const int v_first = cost(tid, s_first, rb_first), all_first = block_scan(v_first, before_first);
+    total = (long long)all_first * a.kv.n_kv;
+    for (int p0 = kPrThreads; p0 < n_pairs; p0 += kPrThreads) {
+        int s, rb;
+        total += (long long)block_scan(cost(p0 + tid, s, rb), before) * a.kv.n_kv;
     }
     const long long want = (total + a.min_tiles - 1) / a.min_tiles;
     const long long nw = max(1LL, want < gridDim.x ? want : gridDim.x);
-    const long long each = total / nw, more = total - each * nw;
-    const long long c0 = blockIdx.x * each + min((long long)blockIdx.x, more);
-    const long long c1 = c0 + each + (blockIdx.x < more ? 1 : 0);
-    const bool work = blockIdx.x < nw && c1 > c0;
+    p.share.each = total / nw;
+    p.share.more = total - p.share.each * nw;
+    const long long c0 = blockIdx.x * p.share.each + min((long long)blockIdx.x, p.share.more);
+    p.share.end = c0 + p.share.each + (blockIdx.x < p.share.more ? 1 : 0);
+    bool work = blockIdx.x < nw && p.share.end > c0;
     PromptSeg seg = {};
-    volatile int * found = reinterpret_cast<volatile int *>(gen + HDR + 336); // s, rb, head, tile
+    volatile int * found = reinterpret_cast<volatile int *>(gen + HDR + 336); // s, rb, head, position in the unit
     if (work) {
         long long run = 0;
         for (int p0 = 0; p0 < n_pairs; p0 += kPrThreads) {
-            int v = 0, s = 0, rb = 0;
-            if (p0 + tid < n_pairs) {
-                find(p0 + tid, s, rb);
-                v = p.unit(s, rb).k.count;
+            int v = v_first, s = s_first, rb = rb_first, all = all_first;
+            before = before_first;
+            if (p0 > 0) {
+                v = cost(p0 + tid, s, rb);
+                all = block_scan(v, before);
             }
-            const int all = block_scan(v, before);
             const long long b = run + (long long)before * a.kv.n_kv;
             if (v > 0 && c0 >= b && c0 < b + (long long)v * a.kv.n_kv) {
                 const int in = (int)(c0 - b);
@@ -740,24 +827,30 @@ template <int T, int D> __global__ void __launch_bounds__(kPrThreads, 1) attn_pr
     __syncthreads();
     tc_fence_after();
     p.tmem = *reinterpret_cast<volatile uint32_t *>(gen + HDR + 328);
+    PromptUnit u = {};
     if (work) {
         seg.s = found[0];
         seg.rb = found[1];
         seg.h = found[2];
-        seg.t_begin = found[3];
-        const PromptUnit u = p.unit(seg.s, seg.rb);
-        const long long left = c1 - c0;
-        const int here = u.k.count - seg.t_begin;
-        seg.t_end = seg.t_begin + (int)(left < here ? left : here);
+        seg.pos = c0 - found[3];
+        u = p.unit(seg.s, seg.rb);
+        seg.t_begin = max(0, found[3] - kPrUnitCost);
+        seg.t_end = (int)min((long long)u.k.count, p.share.end - seg.pos - kPrUnitCost);
+        work = seg.t_end > seg.t_begin; // a share may end inside a unit's fixed cost
+        if (!work && seg.pos + u.k.count + kPrUnitCost < p.share.end) {
+            work = p.advance(seg, u);
+        }
+    }
+    if (work) {
         if (warp < 8) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-            p.softmax(seg, u, left, c0, each, more);
+            p.softmax(seg, u);
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
             if (warp > 8) {
-                p.produce(seg, u, left);
+                p.produce(seg, u);
             } else if (lane == 0) {
-                p.multiply(seg, u, left);
+                p.multiply(seg, u);
             }
         }
     }
