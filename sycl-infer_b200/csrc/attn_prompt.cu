@@ -36,18 +36,32 @@ __host__ __device__ constexpr int pr_smem(int dim) { return (4 + pr_slots(dim)) 
 // floats that a CTA leaves of one 128-row tile: o by column, then m and l
 __host__ __device__ constexpr int pr_part_floats(int dim) { return (dim + 2) * 128; }
 
-// D[tmem] (+)= A B, 16-bit operands, fp32 sums; issued by one thread.  A from shared or from tensor memory.
-__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+// D[tmem] (+)= A B, 16-bit operands, fp32 sums; issued by one thread.  A from shared or from tensor memory.  Descriptors
+// come as the low words of their first product with the shared high word; AO, BO step them (in 16 bytes, or columns), so
+// that the unrolled products of a tile need no more than these registers.
+template <int AO, int BO>
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b32 al, bl;\n\t.reg .b64 ad, bd;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                 "add.u32 al, %1, %7;\n\tadd.u32 bl, %3, %8;\n\tmov.b64 ad, {al, %2};\n\tmov.b64 bd, {bl, %4};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %5, p;\n\t}" ::"r"(d),
+                 "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "n"(AO), "n"(BO)
                  : "memory");
 }
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-                 "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+template <int AO, int BO>
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b32 at, bl;\n\t.reg .b64 bd;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+                 "add.u32 at, %1, %6;\n\tadd.u32 bl, %2, %7;\n\tmov.b64 bd, {bl, %3};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [at], bd, %4, p;\n\t}" ::"r"(d),
+                 "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "n"(AO), "n"(BO)
                  : "memory");
+}
+// f(0), f(1), ... with the index as a constant
+template <int N, int I = 0, class F> __device__ __forceinline__ void unrolled(F && f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        unrolled<N, I + 1>(f);
+    }
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint64_t (&v)[16]) { // 32 columns, in pairs
     uint32_t * u = reinterpret_cast<uint32_t *>(v);
@@ -224,34 +238,26 @@ template <int T, int D> struct Prompt {
         uint32_t p_par = 0, q_par = 0, item = 0; // a bit a tile: the phase that is waited for
         auto s_cols = [&](int t) { return tmem + (uint32_t)t * 128; };
         auto o_cols = [&](int t) { return tmem + 256 + (uint32_t)t * 128; };
-        // the loops stay loops: a product takes longer than its issue, and unrolled descriptors would spill
+        const uint64_t k_desc = smem_desc_sw128(0, 16, 1024);
+        // V as stored is N-major: blocks of 64 values 16384 bytes apart, groups of eight keys 1024
+        const uint64_t v_desc = smem_desc_sw128(0, 16384, 1024);
+        const uint32_t k_hi = (uint32_t)(k_desc >> 32), v_hi = (uint32_t)(v_desc >> 32);
         auto scores = [&](int t, uint32_t slot) { // s = q k: low part first
-            const uint64_t kd = smem_desc_sw128(slot_addr((int)slot), 16, 1024);
-            uint32_t accumulate = 0;
-#pragma unroll 1
-            for (int part = 1; part >= 0; part--) {
-                const uint64_t qd = smem_desc_sw128(q_addr(t, part), 16, 1024);
-#pragma unroll 1
-                for (int ks = 0; ks < KS; ks++) { // 16 values: 32 bytes of a 128-byte row, then the next block of 64
-                    const uint64_t off = (uint64_t)(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
-                    mma_f16_ss(s_cols(t), qd + off, kd + off, id_qk, accumulate);
-                    accumulate = 1;
-                }
-            }
+            const uint32_t qd = (uint32_t)k_desc | q_addr(t, 0) >> 4, kd = (uint32_t)k_desc | slot_addr((int)slot) >> 4, to = s_cols(t);
+            unrolled<2 * KS>([&](auto n) {
+                constexpr int i = decltype(n)::value;
+                // 16 values: 32 bytes of a 128-byte row, then the next block of 64
+                constexpr int part = i < KS ? 1 : 0, ks = i % KS, off = ((ks >> 2) * 16384 + (ks & 3) * 32) >> 4;
+                mma_f16_ss<off + part * (TILE >> 4), off>(to, qd, k_hi, kd, k_hi, id_qk, i > 0);
+            });
         };
         auto values = [&](int t, uint32_t slot) { // o = p v: low part first
-            // V as stored is N-major: blocks of 64 values 16384 bytes apart, groups of eight keys 1024
-            const uint64_t vd = smem_desc_sw128(slot_addr((int)slot), 16384, 1024);
-            uint32_t accumulate = 0;
-#pragma unroll 1
-            for (int part = 1; part >= 0; part--) {
-#pragma unroll 1
-                for (int ks = 0; ks < kPrKeys / 16; ks++) {
-                    const uint32_t p = s_cols(t) + (uint32_t)((ks >> 1) * 32 + (ks & 1) * 8 + part * 16);
-                    mma_f16_ts(o_cols(t), p, vd + (uint64_t)(ks * (2048 >> 4)), id_pv, accumulate);
-                    accumulate = 1;
-                }
-            }
+            const uint32_t vd = (uint32_t)v_desc | slot_addr((int)slot) >> 4, p = s_cols(t), to = o_cols(t);
+            unrolled<kPrKeys / 8>([&](auto n) {
+                constexpr int i = decltype(n)::value;
+                constexpr int part = i < kPrKeys / 16 ? 1 : 0, ks = i % (kPrKeys / 16);
+                mma_f16_ts<(ks >> 1) * 32 + (ks & 1) * 8 + part * 16, ks * (2048 >> 4)>(to, p, vd, v_hi, id_pv, i > 0);
+            });
         };
         auto full = [&](uint32_t it) { wait(bars.kv_full + 8 * (it % SLOTS), (it / SLOTS) & 1); };
         auto release = [&](uint32_t it) { mma_commit(bars.kv_empty + 8 * (it % SLOTS)); };
