@@ -63,18 +63,16 @@ template <int N, int I = 0, class F> __device__ __forceinline__ void unrolled(F 
         unrolled<N, I + 1>(f);
     }
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint64_t (&v)[16]) { // 32 columns, in pairs
-    uint32_t * u = reinterpret_cast<uint32_t *>(v);
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
-                   "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]),
-                   "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]),
-                   "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
-                 : "r"(taddr)
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint64_t (&v)[8]) { // 16 columns, in pairs
+    tmem_ld16(taddr, reinterpret_cast<uint32_t (&)[16]>(v));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&u)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(u[0]), "r"(u[1]), "r"(u[2]),
+                 "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
                  : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&u)[16]) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint64_t (&v)[8]) {
+    const uint32_t * u = reinterpret_cast<const uint32_t *>(v);
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
                  "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
                  "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
@@ -256,7 +254,7 @@ template <int T, int D> struct Prompt {
             unrolled<kPrKeys / 8>([&](auto n) {
                 constexpr int i = decltype(n)::value;
                 constexpr int part = i < kPrKeys / 16 ? 1 : 0, ks = i % (kPrKeys / 16);
-                mma_f16_ts<(ks >> 1) * 32 + (ks & 1) * 8 + part * 16, ks * (2048 >> 4)>(to, p, vd, v_hi, id_pv, i > 0);
+                mma_f16_ts<ks * 16 + part * 8, ks * (2048 >> 4)>(to, p, vd, v_hi, id_pv, i > 0);
             });
         };
         auto full = [&](uint32_t it) { wait(bars.kv_full + 8 * (it % SLOTS), (it / SLOTS) & 1); };
@@ -341,31 +339,39 @@ template <int T, int D> struct Prompt {
                          : "memory");
             return __all_sync(~0u, ok != 0);
         };
-        // the tile's groups of 16 keys, one a lane: where its rows lie and which of them are seen
-        auto look = [&](int tile, unsigned long long & src, uint32_t & seen) {
+        // the tile's groups of 16 keys, one a lane: where its rows lie and which of them are seen.  Looked up a tile ahead of the
+        // copies, with a hint to bring the group into L2.
+        auto look = [&](int i, unsigned long long & src, uint32_t & seen) {
             src = 0;
             seen = 0;
-            if (lane < kPrKeys / 16) {
-                const int k0 = tile * kPrKeys + lane * 16;
+            if (i < x.t_end && lane < kPrKeys / 16) {
+                const int k0 = key_tile(u.k, i) * kPrKeys + lane * 16;
                 seen = keys_seen(u.k, k0, a.n_sink);
                 if (seen) {
                     const int page = a.b.page_table[(size_t)x.s * a.b.table_stride + (k0 >> a.kv.page_shift)];
                     if (page >= 0 && page < a.kv.n_pages) {
                         src = (unsigned long long)page * a.kv.page_bytes +
                               (((unsigned long long)x.h << a.kv.page_shift) + (k0 & ((1 << a.kv.page_shift) - 1))) * ROWB;
+                        if (w == 0) {
+                            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.kv.k + src), "n"(16 * ROWB) : "memory");
+                            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.kv.v + src), "n"(16 * ROWB) : "memory");
+                        }
                     } else {
                         seen = 0;
                         atomicExch(&g_attn_prompt_status, B200Q_EINVAL);
                     }
                 }
             }
+            __syncwarp();
         };
+        const int row = lane / CPR, chunk = lane % CPR; // of a piece
         for (;;) {
+            unsigned long long src, src_next;
+            uint32_t seen, seen_next;
+            look(x.t_begin, src, seen);
             for (int j = x.t_begin; j < x.t_end; j++) {
-                unsigned long long src;
-                uint32_t seen;
-                look(key_tile(u.k, j), src, seen);
-                const uint32_t valid = __ballot_sync(~0u, seen != 0);
+                look(j + 1, src_next, seen_next);
+                const uint32_t valid = __ballot_sync(~0u, seen != 0), full = __ballot_sync(~0u, seen == 0xFFFFu);
                 if (w == 0 && lane == 0) {
                     meta[tile_n & 7] = (int)valid;
                 }
@@ -381,17 +387,26 @@ template <int T, int D> struct Prompt {
                     const uint8_t * pool = kv ? a.kv.v : a.kv.k;
                     const uint32_t dst = slot_addr(slot);
                     if constexpr (T != kE4M3) {
-#pragma unroll 4
-                        for (int i = w; i < PIECES; i += 3) {
-                            const int gr = i / PER_GROUP;
-                            const unsigned long long off = __shfl_sync(~0u, src, gr) + (i % PER_GROUP) * 512 + lane * 16;
-                            const uint32_t rows = __shfl_sync(~0u, seen, gr);
-                            const int r = i * (32 / CPR) + lane / CPR;
-                            const bool take = (rows >> (r & 15)) & 1;
-                            const uint32_t to = dst + sw128_off(r, lane % CPR);
-                            const int n = take ? 16 : 0;
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(take ? pool + off : pool), "r"(n)
-                                         : "memory");
+#pragma unroll 1
+                        for (int gr = w; gr < kPrKeys / 16; gr += 3) {
+                            const uint8_t * from = pool + __shfl_sync(~0u, src, gr) + lane * 16;
+                            const uint32_t to = dst + (uint32_t)gr * 2048;
+                            if ((full >> gr) & 1) {
+#pragma unroll
+                                for (int i = 0; i < PER_GROUP; i++) {
+                                    cp_async16(to + sw128_off(i * (32 / CPR) + row, chunk), from + i * 512);
+                                }
+                            } else { // rows that nobody sees (their memory may hold anything) become zeros
+                                const uint32_t rows = __shfl_sync(~0u, seen, gr);
+#pragma unroll
+                                for (int i = 0; i < PER_GROUP; i++) {
+                                    const bool take = (rows >> (i * (32 / CPR) + row)) & 1;
+                                    const int n = take ? 16 : 0;
+                                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + sw128_off(i * (32 / CPR) + row, chunk)),
+                                                 "l"(take ? from + i * 512 : pool), "r"(n)
+                                                 : "memory");
+                                }
+                            }
                         }
                         cp_async_commit();
                         flush(false);
@@ -404,7 +419,7 @@ template <int T, int D> struct Prompt {
                             const int gr = min(i / PER_GROUP, kPrKeys / 16 - 1);
                             const unsigned long long off = __shfl_sync(~0u, src, gr) + (i % PER_GROUP) * 512 + lane * 16;
                             const uint32_t rows = __shfl_sync(~0u, seen, gr);
-                            const int r = i * (32 / CPR) + lane / CPR;
+                            const int r = i * (32 / CPR) + row;
                             raw[q] = make_uint4(0, 0, 0, 0);
                             if (i < PIECES && ((rows >> (r & 15)) & 1)) {
                                 raw[q] = __ldg(reinterpret_cast<const uint4 *>(pool + off));
@@ -414,7 +429,7 @@ template <int T, int D> struct Prompt {
                         for (int q = 0; q < MINE; q++) {
                             const int i = w + 3 * q;
                             if (i < PIECES) {
-                                const int r = i * (32 / CPR) + lane / CPR, c = lane % CPR * 2;
+                                const int r = i * (32 / CPR) + row, c = chunk * 2;
                                 sts128(dst + sw128_off(r, c), e4m3x2_to_f16x2(raw[q].x), e4m3x2_to_f16x2(raw[q].x >> 16),
                                        e4m3x2_to_f16x2(raw[q].y), e4m3x2_to_f16x2(raw[q].y >> 16));
                                 sts128(dst + sw128_off(r, c + 1), e4m3x2_to_f16x2(raw[q].z), e4m3x2_to_f16x2(raw[q].z >> 16),
@@ -425,6 +440,8 @@ template <int T, int D> struct Prompt {
                         mbar_arrive(bars.kv_full + 8 * slot);
                     }
                 }
+                src = src_next;
+                seen = seen_next;
             }
             if (!advance(x, u)) {
                 break;
@@ -458,10 +475,10 @@ template <int T, int D> struct Prompt {
                 const long long q_at = (long long)(u.r.row0 + tok) * a.q_stride + (long long)head * D;
                 const int d = lane % (32 / RPL) * 4;
 #pragma unroll 1
-                for (int i0 = 0; i0 < 32; i0 += 8 * RPL) {
-                    float4 v[8];
+                for (int i0 = 0; i0 < 32; i0 += 16 * RPL) {
+                    float4 v[16];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
+                    for (int i = 0; i < 16; i++) {
                         const int row = i0 + i * RPL + lane / (32 / RPL);
                         const float * q = a.q + __shfl_sync(~0u, q_at, row) + d;
                         v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -474,7 +491,7 @@ template <int T, int D> struct Prompt {
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
+                    for (int i = 0; i < 16; i++) {
                         const int row = i0 + i * RPL + lane / (32 / RPL);
                         if constexpr (!BF) {
                             float top = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
@@ -510,16 +527,20 @@ template <int T, int D> struct Prompt {
                 }
                 float m = -INFINITY, l = 0.0f, f = 1.0f;
                 const int low = a.window ? pos - a.window + 1 : 0;
+                // A load from tensor memory is waited for only when the next one has been issued.
                 auto add_o = [&]() { // o = o f + the tile's p v
                     const uint64_t ff = pair2(f, f);
+                    uint64_t v[2][8];
+                    tmem_ld16(o_cols, v[0]);
 #pragma unroll
-                    for (int c = 0; c < D / 32; c++) {
-                        uint64_t v[16];
-                        tmem_ld32(o_cols + 32 * c, v);
+                    for (int c = 0; c < D / 16; c++) {
                         tmem_ld_wait();
+                        if (c + 1 < D / 16) {
+                            tmem_ld16(o_cols + 16 * (c + 1), v[(c + 1) & 1]);
+                        }
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            o[16 * c + i] = fma2(o[16 * c + i], ff, v[i]);
+                        for (int i = 0; i < 8; i++) {
+                            o[8 * c + i] = fma2(o[8 * c + i], ff, v[c & 1][i]);
                         }
                     }
                 };
@@ -535,32 +556,44 @@ template <int T, int D> struct Prompt {
                     const uint32_t valid = (uint32_t)meta[(tile_n + j) & 7];
                     const bool whole = valid == 0xFFu && key0 + kPrKeys - 1 <= pos_min &&
                                        (a.window == 0 || key0 > pos_max - a.window || key0 + kPrKeys <= a.n_sink);
-                    // columns that the row sees, of 32 from column c on
+                    // columns that the row sees, of the 16 (one group) from column c on
                     auto seen = [&](int c) {
-                        auto below = [](int k) { return k >= 32 ? ~0u : (k <= 0 ? 0u : (1u << k) - 1u); }; // bits 0 .. k-1
-                        const uint32_t groups = ((valid >> (c / 16)) & 1 ? 0xFFFFu : 0u) | ((valid >> (c / 16 + 1)) & 1 ? 0xFFFF0000u : 0u);
-                        return groups & below(pos + 1 - key0 - c) & (~below(low - key0 - c) | below(a.n_sink - key0 - c));
+                        auto below = [](int k) { return k >= 16 ? 0xFFFFu : (k <= 0 ? 0u : (1u << k) - 1u); }; // bits 0 .. k-1
+                        const uint32_t bits = below(pos + 1 - key0 - c) & (~below(low - key0 - c) | below(a.n_sink - key0 - c));
+                        return (valid >> (c / 16)) & 1 ? bits : 0u;
                     };
-                    auto load = [&](int c, uint64_t (&v)[16]) {
-                        tmem_ld32(s_cols + c, v);
-                        tmem_ld_wait();
-                        if (!whole) {
+                    float top = -INFINITY;
+                    auto look = [&](int c, uint64_t (&v)[8]) {
+                        if (!whole) { // masked scores go back: the second reading needs no masks
                             const uint32_t bits = seen(c);
 #pragma unroll
-                            for (int i = 0; i < 16; i++) {
+                            for (int i = 0; i < 8; i++) {
                                 v[i] = pair2((bits >> (2 * i)) & 1 ? first2(v[i]) : -INFINITY,
                                              (bits >> (2 * i + 1)) & 1 ? second2(v[i]) : -INFINITY);
                             }
+                            tmem_st16(s_cols + c, v);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            top = fmaxf(top, fmaxf(first2(v[i]), second2(v[i])));
                         }
                     };
-                    float top = -INFINITY;
+                    {
+                        uint64_t v[2][8];
+                        tmem_ld16(s_cols, v[0]);
 #pragma unroll 1
-                    for (int c = 0; c < kPrKeys; c += 32) {
-                        uint64_t v[16];
-                        load(c, v);
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            top = fmaxf(top, fmaxf(first2(v[i]), second2(v[i])));
+                        for (int c = 0; c < kPrKeys; c += 32) {
+                            tmem_ld_wait();
+                            tmem_ld16(s_cols + c + 16, v[1]);
+                            look(c, v[0]);
+                            tmem_ld_wait();
+                            if (c + 32 < kPrKeys) {
+                                tmem_ld16(s_cols + c + 32, v[0]);
+                            }
+                            look(c + 16, v[1]);
+                        }
+                        if (!whole) {
+                            tmem_st_wait();
                         }
                     }
                     const float mn = fmaxf(m, top * cq);
@@ -569,13 +602,10 @@ template <int T, int D> struct Prompt {
                     m = mn;
                     uint64_t sum = 0, sum1 = 0;
                     const uint64_t cc = pair2(cq, cq), oo = pair2(off, off);
-#pragma unroll 1
-                    for (int c = 0; c < kPrKeys; c += 32) {
-                        uint64_t v[16];
-                        load(c, v);
-                        uint32_t hi[16], lo[16];
+                    auto weigh = [&](int c, const uint64_t (&v)[8]) { // p of 16 keys takes the place of their s
+                        uint32_t hi[8], lo[8];
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
+                        for (int i = 0; i < 8; i++) {
                             const uint64_t e = fma2(v[i], cc, oo);
                             const float p0 = exp2_fast(first2(e)), p1 = exp2_fast(second2(e));
                             const uint64_t pp = pair2(p0, p1);
@@ -589,8 +619,23 @@ template <int T, int D> struct Prompt {
                             hi[i] = part[0];
                             lo[i] = part[1];
                         }
-                        tmem_st16(s_cols + c, hi); // over the 32 columns of s that were just read
-                        tmem_st16(s_cols + c + 16, lo);
+                        tmem_st8(s_cols + c, hi);
+                        tmem_st8(s_cols + c + 8, lo);
+                    };
+                    {
+                        uint64_t v[2][8];
+                        tmem_ld16(s_cols, v[0]);
+#pragma unroll 1
+                        for (int c = 0; c < kPrKeys; c += 32) {
+                            tmem_ld_wait();
+                            tmem_ld16(s_cols + c + 16, v[1]);
+                            weigh(c, v[0]);
+                            tmem_ld_wait();
+                            if (c + 32 < kPrKeys) {
+                                tmem_ld16(s_cols + c + 32, v[0]);
+                            }
+                            weigh(c + 16, v[1]);
+                        }
                     }
                     sum = add2(sum, sum1);
                     l = fmaf(l, f_new, first2(sum) + second2(sum));
