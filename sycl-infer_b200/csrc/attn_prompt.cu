@@ -150,7 +150,7 @@ struct PromptUnit {
 };
 // A CTA's share of the list is measured in tiles plus kPrUnitCost a unit (its q, its join, its rows out): tile i of a unit
 // that starts at position `pos` of the list lies at pos + kPrUnitCost + i.
-constexpr int kPrUnitCost = 1;
+constexpr int kPrUnitCost = 3;
 struct PromptSeg {
     int s, h, rb;
     int t_begin, t_end;
@@ -365,7 +365,20 @@ template <int T, int D> struct Prompt {
             __syncwarp();
         };
         const int row = lane / CPR, chunk = lane % CPR; // of a piece
+        // the next unit's q towards L2 while this one runs: a token's heads of the group lie together
+        auto hint_q = [&]() {
+            PromptSeg y = x;
+            PromptUnit v = u;
+            if (w == 1 && a.vec && advance(y, v)) {
+                const int t0 = v.row0 / a.group, t1 = (v.row0 + v.rows - 1) / a.group;
+                for (int i = t0 + lane; i <= t1; i += 32) {
+                    const float * q = a.q + (size_t)(v.r.row0 + i) * a.q_stride + (size_t)y.h * a.group * D;
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(q), "r"(a.group * D * 4) : "memory");
+                }
+            }
+        };
         for (;;) {
+            hint_q();
             unsigned long long src, src_next;
             uint32_t seen, seen_next;
             look(x.t_begin, src, seen);
