@@ -33,7 +33,7 @@ size_t attn_prompt_part_bytes(int head_dim);
 cudaError_t read_attn_prompt_status(int * status, bool clear);
 cudaError_t launch_attn_decode(cudaStream_t s, AttnDev a);
 size_t attn_decode_units(int n_head, int n_kv, int n_seq, int max_q);
-size_t attn_decode_part_bytes(int n_head, int n_kv, int head_dim, int max_q);
+size_t attn_decode_part_bytes(int n_head, int n_kv, int head_dim, int n_seq, int max_q);
 
 #ifdef __CUDACC__
 

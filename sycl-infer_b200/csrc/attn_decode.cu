@@ -32,11 +32,14 @@ namespace b200q {
 
 __device__ int g_attn_status = 0;
 
-constexpr int kDecWarps = 4;
-constexpr int kDecThreads = kDecWarps * 32;
-constexpr int kDecStages = 3;
 constexpr int kDecStageBytes = 8192; // K and V halves of one tile
-constexpr int kDecPerSM = 2;
+constexpr int kDecTeam = 8;          // warps of a CTA that work on one piece
+// TEAM 1: four warps a CTA, two CTAs an SM with rings of three stages; eight rows of 64 values leave registers for a third
+// CTA, with rings of two (192 x window 1024 keys e4m3: 70 -> 63 us; with 128 values it spills: 73 -> 76 us).
+// TEAM 8: one CTA an SM.
+__host__ __device__ constexpr int dec_warps(int team) { return team == 1 ? 4 : team; }
+__host__ __device__ constexpr int dec_per_sm(int dim, bool h8, int team) { return team > 1 ? 1 : (h8 && dim == 64 ? 3 : 2); }
+__host__ __device__ constexpr int dec_stages(int dim, bool h8, int team) { return team == 1 && h8 && dim == 64 ? 2 : 3; }
 
 // 16-byte chunk `c` of row `r` in a tile of ROWB-byte rows.  16-bit rows are read by ldmatrix (eight rows of one
 // chunk column): chunk ^ row.  8-bit rows are read as fragments, for K four chunks of two neighbouring rows, for V
@@ -112,7 +115,7 @@ __host__ __device__ constexpr int part_floats(int dim, bool h8) { return (dim / 
 
 // H8: at most eight rows a unit, first and second parts side by side in one product; otherwise sixteen rows.
 template <int T, int D, bool H8, int TEAM>
-__global__ void __launch_bounds__(kDecThreads, kDecPerSM) attn_decode_kernel(const __grid_constant__ AttnDev a) {
+__global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM)) attn_decode_kernel(const __grid_constant__ AttnDev a) {
     constexpr int EB = KvElem<T>::BYTES, ROWB = D * EB, KT = kDecStageBytes / 2 / ROWB;
     constexpr int ROWS = H8 ? 8 : 16, KS = D / 16, NT = D / 8;
     constexpr int PARTS = T == kBF16 ? 3 : 2;  // 16-bit parts of q and p
@@ -124,13 +127,14 @@ __global__ void __launch_bounds__(kDecThreads, kDecPerSM) attn_decode_kernel(con
     constexpr int RX = H8 ? 1 : 2;             // rows of a thread
     constexpr float kPBias = T == kBF16 ? 0.0f : 14.0f;
     constexpr int PART = part_floats(D, H8);
+    constexpr int WARPS = dec_warps(TEAM), THREADS = WARPS * 32, STAGES = dec_stages(D, H8, TEAM);
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long s_sum[kDecWarps], s_before[kDecWarps];
-    __shared__ int s_seq[kDecWarps], s_last;
-    __shared__ int2 s_meta[kDecWarps][kDecStages];
+    __shared__ long long s_sum[WARPS], s_before[WARPS];
+    __shared__ int s_seq[WARPS], s_last;
+    __shared__ int2 s_meta[WARPS][STAGES];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * kDecStages * kDecStageBytes;
-    float * join = reinterpret_cast<float *>(smem + kDecWarps * kDecStages * kDecStageBytes); // TEAM 4: two parts
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * kDecStageBytes;
+    float * join = reinterpret_cast<float *>(smem + WARPS * STAGES * kDecStageBytes); // TEAM 4: two parts
 
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -150,7 +154,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecPerSM) attn_decode_kernel(con
         __syncthreads();
         long long all = 0, mine = 0;
 #pragma unroll
-        for (int w = 0; w < kDecWarps; w++) {
+        for (int w = 0; w < WARPS; w++) {
             mine += w < warp ? s_sum[w] : 0;
             all += s_sum[w];
         }
@@ -168,60 +172,115 @@ __global__ void __launch_bounds__(kDecThreads, kDecPerSM) attn_decode_kernel(con
     long long before_first, before;
     long long total = block_sum(v_first, before_first);
     const long long sum_first = total;
-    for (int s0 = kDecThreads; s0 < a.b.n_seq; s0 += kDecThreads) {
+    for (int s0 = THREADS; s0 < a.b.n_seq; s0 += THREADS) {
         total += block_sum(seq_total(s0 + tid), before);
     }
     if (total == 0) {
         return;
     }
-    constexpr int WORKERS = kDecWarps / TEAM; // of a CTA
-    const long long want = (total + a.min_tiles - 1) / a.min_tiles, most = (long long)gridDim.x * WORKERS;
-    const long long nw = want < most ? want : most;
+    // TEAM 1: the list is cut into equal shares, one a warp, wherever the cuts fall; worker w's share starts at
+    // w * each + min(w, more).  TEAM 8: every unit is cut into pieces of equal length, at most `each` tiles, so that a CTA
+    // has one piece of one unit and its way to the end is as short as can be.
+    constexpr int WORKERS = WARPS / TEAM; // of a CTA
+    long long nw, each, more = 0;
+    auto pieces = [&](const SeqTiles & q) { return (int)((q.k.count + each - 1) / each); };
+    auto seq_workers = [&](int s) -> long long { // TEAM 8
+        if (s >= a.b.n_seq) {
+            return 0;
+        }
+        const SeqTiles q = seq_tiles<KT, ROWS>(a, s);
+        return (long long)q.blocks * a.kv.n_kv * pieces(q);
+    };
+    if constexpr (TEAM == 1) {
+        const long long most = (long long)gridDim.x * WORKERS;
+        nw = total < most ? total : most;
+        each = total / nw;
+        more = total - each * nw;
+    } else {
+        long long units = 0;
+        for (int s0 = 0; s0 < a.b.n_seq; s0 += THREADS) {
+            const int s = s0 + tid;
+            units += block_sum(s < a.b.n_seq ? (long long)seq_tiles<KT, ROWS>(a, s).blocks * a.kv.n_kv : 0, before);
+        }
+        // pieces of `each` tiles are at most total / each + units in number
+        each = units < gridDim.x ? (total + gridDim.x - units - 1) / (gridDim.x - units) : total;
+        each = each > TEAM ? each : TEAM; // a tile for every warp
+        nw = 0;
+        for (int s0 = 0; s0 < a.b.n_seq; s0 += THREADS) {
+            nw += block_sum(seq_workers(s0 + tid), before);
+        }
+    }
     if ((long long)blockIdx.x * WORKERS >= nw) {
         return;
     }
-    const int worker = blockIdx.x * WORKERS + warp / TEAM;
-    const long long c0 = worker * total / nw, c1 = (worker + 1) * total / nw;
+    auto share = [&](int w) { return w * each + (w < more ? w : more); };
+    const int w_first = TEAM == 1 ? 0 : warp; // the warp's first tile of a segment
+    const int copy_row = lane / CPR, copy_chunk = lane % CPR;
+    for (int worker = blockIdx.x * WORKERS + warp / TEAM;; worker += (int)gridDim.x * WORKERS) {
+    if (TEAM > 1 && worker >= nw) {
+        break;
+    }
+    // ---- where the worker starts
     {
         long long run = 0;
-        for (int s0 = 0; s0 < a.b.n_seq; s0 += kDecThreads) {
-            long long v = v_first, all = sum_first;
-            before = before_first;
-            if (s0 > 0) {
-                v = seq_total(s0 + tid);
+        for (int s0 = 0; s0 < a.b.n_seq; s0 += THREADS) {
+            long long v, all;
+            if constexpr (TEAM == 1) {
+                v = v_first, all = sum_first, before = before_first;
+                if (s0 > 0) {
+                    v = seq_total(s0 + tid);
+                    all = block_sum(v, before);
+                }
+            } else {
+                v = seq_workers(s0 + tid);
                 all = block_sum(v, before);
             }
+            long long c_last = 0;
 #pragma unroll
             for (int w = 0; w < WORKERS; w++) {
-                const long long c = (blockIdx.x * WORKERS + w) * total / nw;
+                const long long c = TEAM == 1 ? share(blockIdx.x * WORKERS + w) : worker;
                 if (v > 0 && c >= run + before && c < run + before + v) {
                     s_seq[w] = s0 + tid;
                     s_before[w] = run + before;
                 }
+                c_last = c;
             }
             run += all;
-            if (run > (blockIdx.x * WORKERS + WORKERS - 1) * total / nw) {
+            if (run > c_last) {
                 break;
             }
         }
         __syncthreads();
     }
-    if (worker >= nw) {
-        return; // TEAM 1 only: no block barrier from here on
+    if (TEAM == 1 && worker >= nw) {
+        return; // no block barrier from here on
     }
     // the first unit
+    const long long c0 = TEAM == 1 ? share(worker) : 0, c1 = TEAM == 1 ? share(worker + 1) : 1;
     Segment first;
+    int piece = 0, n_pieces = 1; // TEAM 8
+    SeqTiles pq;
     {
         first.s = s_seq[warp / TEAM];
-        const SeqTiles q = seq_tiles<KT, ROWS>(a, first.s);
-        const long long at = c0 - s_before[warp / TEAM];
-        const int u = (int)(at / q.k.count);
-        first.h = u / q.blocks;
-        first.rb = u % q.blocks;
-        first.t_unit = q.k.count;
-        first.t_begin = (int)(at - (long long)u * q.k.count);
-        const long long left = c1 - c0, here = q.k.count - first.t_begin;
-        first.t_end = first.t_begin + (int)(left < here ? left : here);
+        pq = seq_tiles<KT, ROWS>(a, first.s);
+        first.t_unit = pq.k.count;
+        if constexpr (TEAM == 1) {
+            const long long at = c0 - s_before[warp / TEAM];
+            const int u = (int)(at / pq.k.count);
+            first.h = u / pq.blocks;
+            first.rb = u % pq.blocks;
+            first.t_begin = (int)(at - (long long)u * pq.k.count);
+            const long long left = c1 - c0, here = pq.k.count - first.t_begin;
+            first.t_end = first.t_begin + (int)(left < here ? left : here);
+        } else {
+            n_pieces = pieces(pq);
+            const int at = (int)(worker - s_before[0]), u = at / n_pieces;
+            piece = at - u * n_pieces;
+            first.h = u / pq.blocks;
+            first.rb = u % pq.blocks;
+            first.t_begin = (int)((long long)piece * pq.k.count / n_pieces);
+            first.t_end = (int)((long long)(piece + 1) * pq.k.count / n_pieces);
+        }
     }
     // the unit after x, with `left` tiles of the share still to come (> 0)
     auto advance = [&](Segment & x, long long left, SeqTiles & q) {
@@ -239,19 +298,17 @@ __global__ void __launch_bounds__(kDecThreads, kDecPerSM) attn_decode_kernel(con
         x.t_begin = 0;
         x.t_end = (int)(left < q.k.count ? left : q.k.count);
     };
-    const int w_first = TEAM == 1 ? 0 : warp; // the warp's first tile of a segment
 
     // ---- the warp's stream: issue() copies the warp's next tile into the next stage
     Segment ps = first;
-    SeqTiles pq = seq_tiles<KT, ROWS>(a, ps.s);
+    const SeqTiles fq = pq;
     long long p_left = c1 - c0; // tiles from the start of ps on
     int p_tile = ps.t_begin + w_first;
     int p_stage = 0;
-    const int copy_row = lane / CPR, copy_chunk = lane % CPR;
     auto issue = [&]() {
         while (p_tile >= ps.t_end) {
             p_left -= ps.t_end - ps.t_begin;
-            if (p_left <= 0) {
+            if (TEAM > 1 || p_left <= 0) { // a piece is all that a team has
                 cp_async_commit();
                 return;
             }
@@ -305,17 +362,17 @@ __global__ void __launch_bounds__(kDecThreads, kDecPerSM) attn_decode_kernel(con
             }
         }
         cp_async_commit();
-        p_stage = p_stage + 1 == kDecStages ? 0 : p_stage + 1;
+        p_stage = p_stage + 1 == STAGES ? 0 : p_stage + 1;
         p_tile += TEAM;
     };
 #pragma unroll
-    for (int i = 0; i < kDecStages - 1; i++) {
+    for (int i = 0; i < STAGES - 1; i++) {
         issue();
     }
 
     // ---- the units, one after the other
     Segment sg = first;
-    SeqTiles sq = seq_tiles<KT, ROWS>(a, sg.s);
+    SeqTiles sq = fq;
     long long left = c1 - c0, at = c0;
     int stage = 0;
     for (;;) {
@@ -415,12 +472,12 @@ __global__ void __launch_bounds__(kDecThreads, kDecPerSM) attn_decode_kernel(con
 
         for (int i = sg.t_begin + w_first; i < sg.t_end; i += TEAM) {
             issue();
-            cp_async_wait<kDecStages - 1>();
+            cp_async_wait<STAGES - 1>();
             __syncwarp();
             const int2 meta = s_meta[warp][stage];
             const int key0 = meta.x;
             const uint32_t sk = ring + stage * kDecStageBytes, sv = sk + kDecStageBytes / 2;
-            stage = stage + 1 == kDecStages ? 0 : stage + 1;
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
             // ---- s = q . k, the smallest parts first
             float sc[KT / 8][4];
 #pragma unroll
@@ -632,23 +689,19 @@ __global__ void __launch_bounds__(kDecThreads, kDecPerSM) attn_decode_kernel(con
                 v[j] = v[j] * fa[x] + p[j * 32 + lane] * fb[x];
             }
         };
-        auto join_team = [&]() { // the team's first warp ends with all
+        // The team's first warp ends with all: halves of the team put their parts where the warp that takes them has
+        // taken from before, so that one barrier a step is enough.
+        auto join_team = [&]() {
             if constexpr (TEAM > 1) {
-                __syncthreads();
-                if (warp >= 2) {
-                    put(join + (warp - 2) * PART);
-                }
-                __syncthreads();
-                if (warp < 2) {
-                    take(join + warp * PART);
-                }
-                __syncthreads();
-                if (warp == 1) {
-                    put(join);
-                }
-                __syncthreads();
-                if (warp == 0) {
-                    take(join);
+#pragma unroll
+                for (int half = TEAM / 2; half > 0; half >>= 1) {
+                    if (warp >= half && warp < 2 * half) {
+                        put(join + (2 * half == TEAM ? warp - half : warp) * PART);
+                    }
+                    __syncthreads();
+                    if (warp < half) {
+                        take(join + (2 * half == TEAM ? warp : warp + half) * PART);
+                    }
                 }
             }
         };
@@ -656,13 +709,21 @@ __global__ void __launch_bounds__(kDecThreads, kDecPerSM) attn_decode_kernel(con
         join_team();
         bool write = true;
         if (sg.t_end - sg.t_begin != sg.t_unit) {
-            // the unit spans workers: its tiles are [u0, u0 + t_unit) of the list
-            const long long u0 = at - sg.t_begin;
-            auto owner = [&](long long x) { return (int)(((x + 1) * nw - 1) / total); };
-            const int b0 = owner(u0), b1 = owner(u0 + sg.t_unit - 1);
+            // the unit spans workers
+            int b0, b1;
+            if constexpr (TEAM == 1) { // its tiles are [u0, u0 + t_unit) of the list
+                const long long u0 = at - sg.t_begin;
+                auto owner = [&](long long x) { // the worker whose share holds tile x
+                    return (int)(x < more * (each + 1) ? x / (each + 1) : more + (x - more * (each + 1)) / each);
+                };
+                b0 = owner(u0), b1 = owner(u0 + sg.t_unit - 1);
+            } else {
+                b0 = worker - piece, b1 = b0 + n_pieces - 1;
+            }
+            // of a worker's two slots (TEAM 8: one) the second holds the unit that starts in its share and runs on behind it
+            auto slot = [&](int b, bool starts) { return a.parts + (TEAM == 1 ? (size_t)b * 2 + (starts ? 1 : 0) : (size_t)b) * PART; };
             if (lead) {
-                // of a worker's two slots the second holds the unit that starts in its share and runs on behind it
-                put(a.parts + ((size_t)worker * 2 + (sg.t_begin == 0 ? 1 : 0)) * PART);
+                put(slot(worker, sg.t_begin == 0));
                 __threadfence();
                 __syncwarp();
                 uint32_t last = 0;
@@ -694,7 +755,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecPerSM) attn_decode_kernel(con
                     v[j] = 0.0f;
                 }
                 for (int b = b0 + w_first; b <= b1; b += TEAM) {
-                    take(a.parts + ((size_t)b * 2 + (b == b0 ? 1 : 0)) * PART);
+                    take(slot(b, b == b0));
                 }
                 join_team();
             }
@@ -718,23 +779,28 @@ __global__ void __launch_bounds__(kDecThreads, kDecPerSM) attn_decode_kernel(con
         }
         left -= sg.t_end - sg.t_begin;
         at += sg.t_end - sg.t_begin;
-        if (left <= 0) {
+        if (TEAM > 1 || left <= 0) {
             break;
         }
         advance(sg, left, sq);
     }
     cp_async_wait<0>();
+    if constexpr (TEAM == 1) {
+        return;
+    }
+    __syncthreads(); // s_seq and the join space are used again
+    }
 }
 
-template <int T, int D, bool H8, int TEAM> static cudaError_t launch_t(cudaStream_t s, const AttnDev & a, int grid) {
-    constexpr int smem = kDecWarps * kDecStages * kDecStageBytes + (TEAM > 1 ? 2 * part_floats(D, H8) * 4 : 0);
+template <int T, int D, bool H8, int TEAM> static cudaError_t launch_t(cudaStream_t s, const AttnDev & a) {
+    constexpr int smem = dec_warps(TEAM) * dec_stages(D, H8, TEAM) * kDecStageBytes + (TEAM > 1 ? TEAM / 2 * part_floats(D, H8) * 4 : 0);
     const cudaError_t e = ensure_dynamic_smem((const void *)attn_decode_kernel<T, D, H8, TEAM>, smem);
     if (e != cudaSuccess) {
         return e;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(kDecThreads);
+    cfg.gridDim = dim3((unsigned)(kSMs * dec_per_sm(D, H8, TEAM)));
+    cfg.blockDim = dim3(dec_warps(TEAM) * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -745,33 +811,59 @@ template <int T, int D, bool H8, int TEAM> static cudaError_t launch_t(cudaStrea
     return cudaLaunchKernelEx(&cfg, attn_decode_kernel<T, D, H8, TEAM>, a);
 }
 
-constexpr int kDecGrid = kSMs * kDecPerSM;
-
-static int dec_rows(int group, int max_q) { return group * max_q <= 8 ? 8 : 16; }
-// With fewer units than this a team of four warps shares a unit's tiles.
-constexpr size_t kTeamUnits = 128;
-
-size_t attn_decode_units(int n_head, int n_kv, int n_seq, int max_q) {
-    const int rows = dec_rows(n_head / n_kv, max_q);
-    return (size_t)n_seq * n_kv * (((size_t)max_q * (n_head / n_kv) + rows - 1) / rows);
+// How a call is cut.  Few units: teams, so that a unit is left in few parts (B200, f16, 128 values, 8 KV heads: 2, 4, 8, 16
+// sequences of up to 8192 keys 30, 31, 46, 62 us with teams of four, 71, 41, 48, 61 us with warps alone).
+// Rows: as many as there are, up to eight or up to sixteen; e4m3 in many units takes eight in any case, since its
+// conversions and not its bytes bound it and many sequences have fewer rows than the largest (192 x window 1024 keys,
+// 4 to 12 rows: 88 -> 70 us; sixteen rows in all: 116 against 117 us).
+struct DecodeCut {
+    int rows, row_blocks;
+    bool team;
+    size_t units;
+};
+constexpr size_t kTeamUnits = 65;
+static DecodeCut decode_cut(int type, int group, int n_kv, int n_seq, int max_q) {
+    DecodeCut c;
+    const int all = group * max_q;
+    c.rows = all <= 8 ? 8 : 16;
+    c.team = (size_t)n_seq * n_kv < kTeamUnits;
+    if (type == kE4M3 && !c.team) {
+        c.rows = 8;
+    }
+    c.row_blocks = (all + c.rows - 1) / c.rows;
+    c.units = (size_t)n_seq * n_kv * c.row_blocks;
+    return c;
 }
-size_t attn_decode_part_bytes(int n_head, int n_kv, int head_dim, int max_q) {
-    const int rows = dec_rows(n_head / n_kv, max_q);
-    return (size_t)kDecGrid * kDecWarps * 2 * part_floats(head_dim, rows == 8) * sizeof(float);
+
+// for every cut that a call of this shape can get (the cache's type is not known here)
+size_t attn_decode_units(int n_head, int n_kv, int n_seq, int max_q) {
+    return decode_cut(kE4M3, n_head / n_kv, n_kv, n_seq, max_q).units;
+}
+size_t attn_decode_part_bytes(int n_head, int n_kv, int head_dim, int n_seq, int max_q) {
+    size_t most = 0;
+    for (int type : {kF16, kE4M3}) {
+        const DecodeCut c = decode_cut(type, n_head / n_kv, n_kv, n_seq, max_q);
+        const int team = c.team ? kDecTeam : 1;
+        const size_t slots = (size_t)kSMs * dec_per_sm(head_dim, c.rows == 8, team) * (c.team ? 1 : 2 * dec_warps(1));
+        const size_t bytes = slots * part_floats(head_dim, c.rows == 8) * sizeof(float);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
 }
 
 cudaError_t launch_attn_decode(cudaStream_t s, AttnDev a) {
-    const int rows = dec_rows(a.group, a.b.max_q);
-    a.row_blocks = (a.b.max_q * a.group + rows - 1) / rows;
-    const size_t units = (size_t)a.b.n_seq * a.kv.n_kv * a.row_blocks;
-    const bool team = units < kTeamUnits;
-    a.min_tiles = team ? kDecWarps : 1;
+    const DecodeCut c = decode_cut(a.kv.type, a.group, a.kv.n_kv, a.b.n_seq, a.b.max_q);
+    a.row_blocks = c.row_blocks;
     auto go = [&](auto t, auto d) -> cudaError_t {
         constexpr int T = decltype(t)::value, D = decltype(d)::value;
-        if (team) {
-            return rows == 8 ? launch_t<T, D, true, 4>(s, a, kDecGrid) : launch_t<T, D, false, 4>(s, a, kDecGrid);
+        if (c.team) {
+            return c.rows == 8 ? launch_t<T, D, true, kDecTeam>(s, a) : launch_t<T, D, false, kDecTeam>(s, a);
         }
-        return rows == 8 ? launch_t<T, D, true, 1>(s, a, kDecGrid) : launch_t<T, D, false, 1>(s, a, kDecGrid);
+        if constexpr (T == kE4M3) {
+            return launch_t<T, D, true, 1>(s, a);
+        } else {
+            return c.rows == 8 ? launch_t<T, D, true, 1>(s, a) : launch_t<T, D, false, 1>(s, a);
+        }
     };
     auto dim = [&](auto t) {
         return a.kv.head_dim == 64 ? go(t, std::integral_constant<int, 64>{}) : go(t, std::integral_constant<int, 128>{});

@@ -183,7 +183,7 @@ size_t b200q_attn_scratch_bytes(int n_head, int n_kv, int head_dim, int n_seq, i
         return 0;
     }
     const int mq = max_q < n_tok ? max_q : (n_tok > 0 ? n_tok : 1);
-    const size_t parts = (long long)mq * (n_head / n_kv) <= kDecodeRows ? attn_decode_part_bytes(n_head, n_kv, head_dim, mq)
+    const size_t parts = (long long)mq * (n_head / n_kv) <= kDecodeRows ? attn_decode_part_bytes(n_head, n_kv, head_dim, n_seq, mq)
                                                                         : attn_prompt_part_bytes(head_dim);
     return counter_bytes(attn_units(n_head, n_kv, n_seq, mq)) + parts;
 }
