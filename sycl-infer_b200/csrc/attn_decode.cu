@@ -161,12 +161,15 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
         before = mine + x - v;
         return all;
     };
+    // TEAM 8 counts the units along: few, by the rule that chooses it
+    constexpr int kUnitBit = 40;
     auto seq_total = [&](int s) -> long long {
         if (s >= a.b.n_seq) {
             return 0;
         }
         const SeqTiles q = seq_tiles<KT, ROWS>(a, s);
-        return (long long)q.blocks * q.k.count * a.kv.n_kv;
+        const long long units = (long long)q.blocks * a.kv.n_kv;
+        return units * q.k.count + (TEAM > 1 ? units << kUnitBit : 0);
     };
     const long long v_first = seq_total(tid);
     long long before_first, before;
@@ -182,7 +185,7 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
     // w * each + min(w, more).  TEAM 8: every unit is cut into pieces of equal length, at most `each` tiles, so that a CTA
     // has one piece of one unit and its way to the end is as short as can be.
     constexpr int WORKERS = WARPS / TEAM; // of a CTA
-    long long nw, each, more = 0;
+    long long nw, each, more = 0, v_team = 0, sum_team = 0, before_team = 0;
     auto pieces = [&](const SeqTiles & q) { return (int)((q.k.count + each - 1) / each); };
     auto seq_workers = [&](int s) -> long long { // TEAM 8
         if (s >= a.b.n_seq) {
@@ -197,16 +200,14 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
         each = total / nw;
         more = total - each * nw;
     } else {
-        long long units = 0;
-        for (int s0 = 0; s0 < a.b.n_seq; s0 += THREADS) {
-            const int s = s0 + tid;
-            units += block_sum(s < a.b.n_seq ? (long long)seq_tiles<KT, ROWS>(a, s).blocks * a.kv.n_kv : 0, before);
-        }
+        const long long units = total >> kUnitBit;
+        total &= (1LL << kUnitBit) - 1;
         // pieces of `each` tiles are at most total / each + units in number
         each = units < gridDim.x ? (total + gridDim.x - units - 1) / (gridDim.x - units) : total;
         each = each > TEAM ? each : TEAM; // a tile for every warp
-        nw = 0;
-        for (int s0 = 0; s0 < a.b.n_seq; s0 += THREADS) {
+        v_team = seq_workers(tid);
+        sum_team = nw = block_sum(v_team, before_team);
+        for (int s0 = THREADS; s0 < a.b.n_seq; s0 += THREADS) {
             nw += block_sum(seq_workers(s0 + tid), before);
         }
     }
@@ -232,8 +233,11 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
                     all = block_sum(v, before);
                 }
             } else {
-                v = seq_workers(s0 + tid);
-                all = block_sum(v, before);
+                v = v_team, all = sum_team, before = before_team;
+                if (s0 > 0) {
+                    v = seq_workers(s0 + tid);
+                    all = block_sum(v, before);
+                }
             }
             long long c_last = 0;
 #pragma unroll
@@ -813,6 +817,7 @@ template <int T, int D, bool H8, int TEAM> static cudaError_t launch_t(cudaStrea
 
 // How a call is cut.  Few units: teams, so that a unit is left in few parts (B200, f16, 128 values, 8 KV heads: 2, 4, 8, 16
 // sequences of up to 8192 keys 30, 31, 46, 62 us with teams of four, 71, 41, 48, 61 us with warps alone).
+// (teams of eight: 14, 17, 31 us with 2, 4, 8; 33 against 47 with 9, 59 against 54 with 12.)
 // Rows: as many as there are, up to eight or up to sixteen; e4m3 in many units takes eight in any case, since its
 // conversions and not its bytes bound it and many sequences have fewer rows than the largest (192 x window 1024 keys,
 // 4 to 12 rows: 88 -> 70 us; sixteen rows in all: 116 against 117 us).
@@ -821,7 +826,7 @@ struct DecodeCut {
     bool team;
     size_t units;
 };
-constexpr size_t kTeamUnits = 65;
+constexpr size_t kTeamUnits = kSMs / 2 + 1;
 static DecodeCut decode_cut(int type, int group, int n_kv, int n_seq, int max_q) {
     DecodeCut c;
     const int all = group * max_q;
