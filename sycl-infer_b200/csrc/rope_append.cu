@@ -54,9 +54,22 @@ struct AppendArgs {
     BatchDev b;
 };
 
-// VEC = 4: a thread handles pairs four at a time (half layout: two float4 loads half a rotation apart; interleaved:
-// one float4 holds two pairs); VEC = 1: any alignment and any even n_rot.
-template <int T, int VEC> __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const __grid_constant__ AppendArgs a) {
+// What a block reads first of its inputs, then of the batch: which row it is does not depend on the sequence that owns
+// it, so the rows travel while the sequence, the page and the angles are found.
+//
+// VEC = 4: an item is eight values of a head as two float4: in the rotated part four pairs (half layout: the second float4
+// lies half a rotation behind the first; interleaved: next to it), behind it, and in v, eight neighbours.  VEC = 1: an item is
+// one pair, for any alignment and any even n_rot.
+constexpr int kRopeBatch = 2; // items of a thread in flight (1, 2, 4: 25.6, 24.5, 25.8 us for 2048 tokens)
+
+template <int T, int VEC> struct RopeItem {
+    float u[VEC], v[VEC]; // values d0.. and d1..
+    int d0, d1, pair;     // pair: first rotated pair, or -1
+    bool is_q, is_v;
+    int h;
+};
+
+template <int T, int VEC> __global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const __grid_constant__ AppendArgs a) {
     __shared__ float2 cs[kMaxRot / 2];
     __shared__ int s_seq;
     asm volatile("griddepcontrol.launch_dependents;");
@@ -66,6 +79,44 @@ template <int T, int VEC> __global__ void __launch_bounds__(kRopeThreads) rope_a
     }
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int D = a.head_dim, per = D / (2 * VEC); // items of a head
+    const int rot = a.table ? a.n_rot : 0;
+    const int n_q = a.q ? a.n_head : 0, n_all = n_q + (a.k ? 2 * a.n_kv : 0);
+    const int w0 = blockIdx.y * a.heads_per_block * per, w1 = min((blockIdx.y + 1) * a.heads_per_block, n_all) * per;
+    auto read = [&](int w, RopeItem<T, VEC> & x) {
+        const int h = w / per, e = w - h * per;
+        x.is_q = h < n_q;
+        x.is_v = h >= n_q + a.n_kv;
+        x.h = x.is_q ? h : (x.is_v ? h - n_q - a.n_kv : h - n_q);
+        const int turned = x.is_v ? 0 : rot, half = turned / 2;
+        x.pair = VEC * e < half ? VEC * e : -1;
+        if (x.pair >= 0 && !a.interleaved) {
+            x.d0 = VEC * e;
+            x.d1 = x.d0 + half;
+        } else {
+            x.d0 = 2 * VEC * e;
+            x.d1 = x.d0 + VEC;
+        }
+        const float * p = (x.is_q ? a.q + (size_t)t * a.q_stride : (x.is_v ? a.v + (size_t)t * a.v_stride : a.k + (size_t)t * a.k_stride)) + (size_t)x.h * D;
+        if constexpr (VEC == 4) {
+            const float4 u = *reinterpret_cast<const float4 *>(p + x.d0), v = *reinterpret_cast<const float4 *>(p + x.d1);
+            x.u[0] = u.x, x.u[1] = u.y, x.u[2] = u.z, x.u[3] = u.w;
+            x.v[0] = v.x, x.v[1] = v.y, x.v[2] = v.z, x.v[3] = v.w;
+        } else {
+            x.u[0] = p[x.d0];
+            x.v[0] = p[x.d1];
+        }
+    };
+    RopeItem<T, VEC> item[kRopeBatch];
+    auto read_batch = [&](int w) {
+#pragma unroll
+        for (int i = 0; i < kRopeBatch; i++) {
+            if (w + i * kRopeThreads < w1) {
+                read(w + i * kRopeThreads, item[i]);
+            }
+        }
+    };
+    read_batch(w0 + tid);
     // the sequence that owns row t: every thread looks at its share of the ranges, all loads at once
     for (int s = tid; s < a.b.n_seq; s += kRopeThreads) {
         if (a.b.q_start[s] <= t && t < a.b.q_start[s + 1]) {
@@ -78,9 +129,9 @@ template <int T, int VEC> __global__ void __launch_bounds__(kRopeThreads) rope_a
         return; // behind the last sequence
     }
     const SeqRows r = seq_rows(a.b, a.kv.page_shift, seq);
-    const int i = t - r.row0;
-    const int pos = r.n - r.n_row + i;
-    if (i < 0 || i >= r.n_run || pos < 0) {
+    const int i_tok = t - r.row0;
+    const int pos = r.n - r.n_row + i_tok;
+    if (i_tok < 0 || i_tok >= r.n_run || pos < 0) {
         return;
     }
     if (a.table && tid < a.n_rot / 2) {
@@ -101,115 +152,73 @@ template <int T, int VEC> __global__ void __launch_bounds__(kRopeThreads) rope_a
         }
     }
     __syncthreads();
-    const int D = a.head_dim, per = D / VEC / (VEC == 4 ? 1 : 2); // work items of a head
-    const int rot = a.table ? a.n_rot : 0;
-    const int n_q = a.q ? a.n_head : 0, n_all = n_q + (a.k ? 2 * a.n_kv : 0);
-    const int h0 = blockIdx.y * a.heads_per_block, h1 = min(h0 + a.heads_per_block, n_all);
     const int in_page = pos & ((1 << a.kv.page_shift) - 1);
-    for (int w = h0 * per + tid; w < h1 * per; w += kRopeThreads) {
-        const int h = w / per, e = w - h * per;
-        const bool is_q = h < n_q, is_v = h >= n_q + a.n_kv;
-        const int kh = is_q ? 0 : (is_v ? h - n_q - a.n_kv : h - n_q);
-        if (!is_q && page < 0) {
-            continue;
-        }
-        const float * x = is_q ? a.q + (size_t)t * a.q_stride + (size_t)h * D
-                               : (is_v ? a.v + (size_t)t * a.v_stride : a.k + (size_t)t * a.k_stride) + (size_t)kh * D;
-        const int turned = is_v ? 0 : rot;
-        float * y = a.q_out + (size_t)t * a.q_out_stride + (size_t)h * D;
-        uint8_t * z = nullptr;
-        float inv = 1.0f;
-        if (!is_q) {
-            z = (is_v ? a.kv.v : a.kv.k) + (size_t)page * a.kv.page_bytes +
-                (((size_t)kh << a.kv.page_shift) + in_page) * D * KvElem<T>::BYTES;
-            inv = is_v ? a.kv.v_scale : a.kv.k_scale;
-        }
-        if constexpr (VEC == 4) {
-            // the item's eight values as two runs of four: (d0.., d1..)
-            int d0, d1, c0;
-            const int half = turned / 2;
-            float4 u, v;
-            if (a.interleaved || 4 * e >= turned) { // four neighbouring values, alone
-                d0 = 4 * e;
-                u = *reinterpret_cast<const float4 *>(x + d0);
-                if (d0 < turned) {
-                    c0 = d0 / 2;
-                    const float2 A = cs[c0], B = cs[c0 + 1];
-                    u = make_float4(__fsub_rn(__fmul_rn(u.x, A.x), __fmul_rn(u.y, A.y)),
-                                    __fadd_rn(__fmul_rn(u.x, A.y), __fmul_rn(u.y, A.x)),
-                                    __fsub_rn(__fmul_rn(u.z, B.x), __fmul_rn(u.w, B.y)),
-                                    __fadd_rn(__fmul_rn(u.z, B.y), __fmul_rn(u.w, B.x)));
-                }
-                if (is_q) {
-                    *reinterpret_cast<float4 *>(y + d0) = u;
-                } else {
-                    const uint32_t lo = KvElem<T>::pack2(__fdiv_rn(u.x, inv), __fdiv_rn(u.y, inv));
-                    const uint32_t hi = KvElem<T>::pack2(__fdiv_rn(u.z, inv), __fdiv_rn(u.w, inv));
-                    if constexpr (T == kE4M3) {
-                        *reinterpret_cast<uint32_t *>(z + d0) = lo | hi << 16;
-                    } else {
-                        *reinterpret_cast<uint2 *>(z + d0 * 2) = make_uint2(lo, hi);
-                    }
-                }
-                continue;
-            }
-            // half layout: items of the first half do both halves, those of the second nothing
-            d0 = 4 * e;
-            if (d0 >= half) {
-                continue;
-            }
-            d1 = d0 + half;
-            u = *reinterpret_cast<const float4 *>(x + d0);
-            v = *reinterpret_cast<const float4 *>(x + d1);
-            const float uu[4] = {u.x, u.y, u.z, u.w}, vv[4] = {v.x, v.y, v.z, v.w};
-            float ra[4], rb[4];
+    auto finish = [&](RopeItem<T, VEC> & x) {
+        if (x.pair >= 0) {
+            auto turn = [](float & p, float & q, const float2 c) {
+                const float rp = __fsub_rn(__fmul_rn(p, c.x), __fmul_rn(q, c.y));
+                q = __fadd_rn(__fmul_rn(p, c.y), __fmul_rn(q, c.x));
+                p = rp;
+            };
+            if (VEC == 1 || !a.interleaved) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float2 A = cs[d0 + j];
-                ra[j] = __fsub_rn(__fmul_rn(uu[j], A.x), __fmul_rn(vv[j], A.y));
-                rb[j] = __fadd_rn(__fmul_rn(uu[j], A.y), __fmul_rn(vv[j], A.x));
-            }
-            if (is_q) {
-                *reinterpret_cast<float4 *>(y + d0) = make_float4(ra[0], ra[1], ra[2], ra[3]);
-                *reinterpret_cast<float4 *>(y + d1) = make_float4(rb[0], rb[1], rb[2], rb[3]);
-            } else {
-                uint32_t p[4];
-                p[0] = KvElem<T>::pack2(__fdiv_rn(ra[0], inv), __fdiv_rn(ra[1], inv));
-                p[1] = KvElem<T>::pack2(__fdiv_rn(ra[2], inv), __fdiv_rn(ra[3], inv));
-                p[2] = KvElem<T>::pack2(__fdiv_rn(rb[0], inv), __fdiv_rn(rb[1], inv));
-                p[3] = KvElem<T>::pack2(__fdiv_rn(rb[2], inv), __fdiv_rn(rb[3], inv));
-                if constexpr (T == kE4M3) {
-                    *reinterpret_cast<uint32_t *>(z + d0) = p[0] | p[1] << 16;
-                    *reinterpret_cast<uint32_t *>(z + d1) = p[2] | p[3] << 16;
-                } else {
-                    *reinterpret_cast<uint2 *>(z + d0 * 2) = make_uint2(p[0], p[1]);
-                    *reinterpret_cast<uint2 *>(z + d1 * 2) = make_uint2(p[2], p[3]);
+                for (int j = 0; j < VEC; j++) {
+                    turn(x.u[j], x.v[j], cs[x.pair + j]);
                 }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; j += 2) {
+                    turn(x.u[j], x.u[(j + 1) % VEC], cs[x.pair + j / 2]);
+                    turn(x.v[j], x.v[(j + 1) % VEC], cs[x.pair + VEC / 2 + j / 2]);
+                }
+            }
+        }
+        if (x.is_q) {
+            float * y = a.q_out + (size_t)t * a.q_out_stride + (size_t)x.h * D;
+            if constexpr (VEC == 4) {
+                *reinterpret_cast<float4 *>(y + x.d0) = make_float4(x.u[0], x.u[1], x.u[2], x.u[3]);
+                *reinterpret_cast<float4 *>(y + x.d1) = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
+            } else {
+                y[x.d0] = x.u[0];
+                y[x.d1] = x.v[0];
+            }
+            return;
+        }
+        if (page < 0) {
+            return;
+        }
+        const float scale = x.is_v ? a.kv.v_scale : a.kv.k_scale;
+        uint8_t * z = (x.is_v ? a.kv.v : a.kv.k) + (size_t)page * a.kv.page_bytes +
+                      (((size_t)x.h << a.kv.page_shift) + in_page) * D * KvElem<T>::BYTES;
+        auto pack = [&](float p, float q) { return KvElem<T>::pack2(__fdiv_rn(p, scale), __fdiv_rn(q, scale)); };
+        if constexpr (VEC == 4) {
+            const uint32_t p0 = pack(x.u[0], x.u[1]), p1 = pack(x.u[2], x.u[3]), p2 = pack(x.v[0], x.v[1]), p3 = pack(x.v[2], x.v[3]);
+            if constexpr (T == kE4M3) {
+                *reinterpret_cast<uint32_t *>(z + x.d0) = p0 | p1 << 16;
+                *reinterpret_cast<uint32_t *>(z + x.d1) = p2 | p3 << 16;
+            } else {
+                *reinterpret_cast<uint2 *>(z + x.d0 * 2) = make_uint2(p0, p1);
+                *reinterpret_cast<uint2 *>(z + x.d1 * 2) = make_uint2(p2, p3);
             }
         } else {
-            // one pair an item: rotated pairs first, then neighbours of the part that is not rotated
-            const int half = turned / 2;
-            const int d0 = e < half ? (a.interleaved ? 2 * e : e) : 2 * e;
-            const int d1 = e < half && !a.interleaved ? e + half : d0 + 1;
-            float u = x[d0], v = x[d1];
-            if (e < half) {
-                const float2 A = cs[e];
-                const float ra = __fsub_rn(__fmul_rn(u, A.x), __fmul_rn(v, A.y));
-                v = __fadd_rn(__fmul_rn(u, A.y), __fmul_rn(v, A.x));
-                u = ra;
-            }
-            if (is_q) {
-                y[d0] = u;
-                y[d1] = v;
+            const uint32_t p = pack(x.u[0], x.v[0]);
+            if constexpr (T == kE4M3) {
+                z[x.d0] = (uint8_t)p;
+                z[x.d1] = (uint8_t)(p >> 8);
             } else {
-                const uint32_t p = KvElem<T>::pack2(__fdiv_rn(u, inv), __fdiv_rn(v, inv));
-                if constexpr (T == kE4M3) {
-                    z[d0] = (uint8_t)p;
-                    z[d1] = (uint8_t)(p >> 8);
-                } else {
-                    reinterpret_cast<uint16_t *>(z)[d0] = (uint16_t)p;
-                    reinterpret_cast<uint16_t *>(z)[d1] = (uint16_t)(p >> 16);
-                }
+                reinterpret_cast<uint16_t *>(z)[x.d0] = (uint16_t)p;
+                reinterpret_cast<uint16_t *>(z)[x.d1] = (uint16_t)(p >> 16);
+            }
+        }
+    };
+    for (int w = w0 + tid; w < w1; w += kRopeBatch * kRopeThreads) {
+        if (w != w0 + tid) {
+            read_batch(w);
+        }
+#pragma unroll
+        for (int i = 0; i < kRopeBatch; i++) {
+            if (w + i * kRopeThreads < w1) {
+                finish(item[i]);
             }
         }
     }
@@ -258,7 +267,7 @@ cudaError_t launch_rope_append(cudaStream_t s, const double * table, int n_rot, 
     a.b = b;
     auto ok = [](const void * p, int stride) { return !p || (!((uintptr_t)p & 15) && !(stride & 3)); };
     const bool vec = ok(q, q_stride) && ok(k, k_stride) && ok(v, v_stride) && ok(q_out, q_out_stride) &&
-                     (!table || n_rot % (interleaved ? 4 : 8) == 0);
+                     (!table || n_rot % 8 == 0);
     switch (kv.type) {
     case kF16: return launch_append_t<kF16>(s, a, vec);
     case kBF16: return launch_append_t<kBF16>(s, a, vec);
