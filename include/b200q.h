@@ -355,7 +355,7 @@ typedef struct b200q_kv_cache {
  * n rows has position kv_len[s] - n + i; a row whose position would be negative has none (it is neither
  * appended nor rotated, and attention gives zeros for it).  Key j of sequence s lies in page
  * page_table[s * table_stride + j / page_size].  Rows from q_start[n_seq] on are left as they were.
- * kv_len beyond table_stride * page_size counts as that.  A table entry outside [0, n_pages) that
+ * kv_len beyond table_stride * page_size, or 2^30, counts as that.  A table entry outside [0, n_pages) that
  * a visible key (an appended token) needs: the key is left out (the token not stored), and
  * b200q_device_status reports B200Q_EINVAL. */
 typedef struct b200q_kv_batch {
@@ -396,7 +396,7 @@ int b200q_rope_table(void * stream, const b200q_rope * rope /*host*/, double * t
 /* Rotates q into q_out (q_out may be q), rotates k and stores it with v as the newest tokens of the
  * cache.  q, k, v: fp32 rows of n_head * head_dim, n_kv * head_dim values, as the q|k|v call leaves them
  * (views of one buffer included).  table NULL: no rotation.  q NULL: only the append; k and v NULL (both): only
- * the rotation of q.  Angles are formed in 64 bits, so positions up to 2^31 keep fp32 accuracy.  Values
+ * the rotation of q.  Angles are formed in 64 bits, so far positions keep fp32 accuracy.  Values
  * beyond the range of an F16 or E4M3 cache are stored as its largest finite value; NaN stays NaN. */
 int b200q_rope_append(void * stream, const double * table, const b200q_rope * rope /*host*/, const float * q,
                       int q_stride, int n_head, const float * k, int k_stride, const float * v, int v_stride,
@@ -407,12 +407,15 @@ int b200q_rope_append(void * stream, const double * table, const b200q_rope * ro
  *   out = sum_j w_j v_j,  w = softmax over the visible j of scale * q . k_j,
  * key j of KV head h / (n_head / n_kv) visible when j <= p and (window == 0 or j > p - window or
  * j < n_sink).  Rows without a visible key give zeros.  q, out: fp32, one row a token (views included),
- * out must not overlap q.  K and V are used at full precision; q and the weights are split into two 16-bit
- * parts for the tensor cores (relative error below 2^-17), sums are fp32.  A NaN or an infinity among the
+ * out must not overlap q.  K and V are used as they are stored; q and the weights are split into 16-bit parts
+ * for the tensor cores, off by at most 2^-22 of a value over F16 and E4M3 caches (two parts), 2^-24 over BF16 caches
+ * (three parts) with up to 16 query rows a sequence and KV head (max_q * n_head / n_kv), 2^-16 with more (two
+ * parts); sums are fp32.  A NaN or an infinity among the
  * keys or values that a row sees reaches that row, and may reach other rows of the same sequence in
  * the same call; keys that no row of the sequence sees are never used.
- * scratch: b200q_attn_scratch_bytes bytes, 16-byte aligned, zeroed once when it is allocated (the library leaves
- * its counters zero).  Calls that may overlap on the GPU must not share it. */
+ * scratch: b200q_attn_scratch_bytes bytes (the largest over the calls that use it: it depends on the shape),
+ * 16-byte aligned, zeroed once when it is allocated (the library leaves its counters zero).  Calls of any shapes may
+ * use one scratch in turn; calls that may overlap on the GPU must not share it. */
 typedef struct b200q_attn_opts {
     float scale;     /* 0: 1 / sqrt(head_dim) */
     int32_t window;  /* 0: no window */

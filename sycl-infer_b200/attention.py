@@ -84,8 +84,9 @@ class rope_t:
 
 
 def alloc_attn_scratch(n_head, cache, batch):
-    """Caller-owned scratch of `cuda_backend.attn`: one serves every layer and step of one stream, as long as no
-    step has more sequences or rows than `batch`.  Calls that may overlap must not share it."""
+    """Caller-owned scratch of `cuda_backend.attn`: one serves every layer and step of one stream (how much a call needs
+    depends on its shape: take the largest, attn says when it is too small).  Calls that may overlap must not
+    share it."""
     n = load_lib().attn_scratch_bytes(n_head, cache.n_kv, cache.head_dim, batch.n_seq, batch.n_tok, batch.max_q)
     if n == 0:
         raise ValueError(f"alloc_attn_scratch: unsupported shape ({n_head} heads over {cache.n_kv}, head_dim {cache.head_dim})")

@@ -17,9 +17,8 @@ struct AttnDev {
     float v_scale;
     int32_t window, n_sink;
     float * parts;       // scratch: what CTAs leave of units that they share
-    uint32_t * counters; // scratch: arrivals a unit, zero between calls
-    int32_t row_blocks;  // row blocks of a (sequence, KV head) at most
-    int32_t min_tiles;   // tiles that a CTA gets at least
+    uint32_t * counters; // scratch: arrivals at a unit that workers share, by the worker that has its start; zero between calls
+    int32_t min_tiles;   // prompts: tiles that a CTA gets at least
     int32_t vec;         // rows of q and out can be read and written 16 bytes at a time
 };
 
@@ -27,12 +26,14 @@ struct AttnDev {
 constexpr int kDecodeRows = 16;
 constexpr int kMaxSeqs = 4096; // of one step
 
+// The scratch begins with this many counters, whatever the call: calls of different shapes may use one scratch in turn,
+// and no call's parts ever lie where another keeps its counters.
+constexpr int kAttnCounters = 2048;
+
 cudaError_t launch_attn_prompt(cudaStream_t s, AttnDev a);
-size_t attn_prompt_units(int n_head, int n_kv, int n_seq, int max_q);
 size_t attn_prompt_part_bytes(int head_dim);
 cudaError_t read_attn_prompt_status(int * status, bool clear);
-cudaError_t launch_attn_decode(cudaStream_t s, AttnDev a);
-size_t attn_decode_units(int n_head, int n_kv, int n_seq, int max_q);
+cudaError_t launch_attn_decode(cudaStream_t s, const AttnDev & a);
 size_t attn_decode_part_bytes(int n_head, int n_kv, int head_dim, int n_seq, int max_q);
 
 #ifdef __CUDACC__

@@ -732,7 +732,7 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
                 __syncwarp();
                 uint32_t last = 0;
                 if (lane == 0) {
-                    uint32_t * counter = a.counters + (sg.s * a.kv.n_kv + sg.h) * a.row_blocks + sg.rb;
+                    uint32_t * counter = a.counters + b0; // one unit at most starts in a worker's share and runs on behind it
                     last = atomicAdd(counter, 1u) == (uint32_t)(b1 - b0);
                     if (last) {
                         *counter = 0; // as the next call wants it
@@ -822,10 +822,10 @@ template <int T, int D, bool H8, int TEAM> static cudaError_t launch_t(cudaStrea
 // conversions and not its bytes bound it and many sequences have fewer rows than the largest (192 x window 1024 keys,
 // 4 to 12 rows: 88 -> 70 us; sixteen rows in all: 116 against 117 us).
 struct DecodeCut {
-    int rows, row_blocks;
+    int rows;
     bool team;
-    size_t units;
 };
+static_assert(kSMs * 3 * dec_warps(1) <= kAttnCounters, "a counter for every worker");
 constexpr size_t kTeamUnits = kSMs / 2 + 1;
 static DecodeCut decode_cut(int type, int group, int n_kv, int n_seq, int max_q) {
     DecodeCut c;
@@ -835,15 +835,10 @@ static DecodeCut decode_cut(int type, int group, int n_kv, int n_seq, int max_q)
     if (type == kE4M3 && !c.team) {
         c.rows = 8;
     }
-    c.row_blocks = (all + c.rows - 1) / c.rows;
-    c.units = (size_t)n_seq * n_kv * c.row_blocks;
     return c;
 }
 
 // for every cut that a call of this shape can get (the cache's type is not known here)
-size_t attn_decode_units(int n_head, int n_kv, int n_seq, int max_q) {
-    return decode_cut(kE4M3, n_head / n_kv, n_kv, n_seq, max_q).units;
-}
 size_t attn_decode_part_bytes(int n_head, int n_kv, int head_dim, int n_seq, int max_q) {
     size_t most = 0;
     for (int type : {kF16, kE4M3}) {
@@ -856,9 +851,8 @@ size_t attn_decode_part_bytes(int n_head, int n_kv, int head_dim, int n_seq, int
     return most;
 }
 
-cudaError_t launch_attn_decode(cudaStream_t s, AttnDev a) {
+cudaError_t launch_attn_decode(cudaStream_t s, const AttnDev & a) {
     const DecodeCut c = decode_cut(a.kv.type, a.group, a.kv.n_kv, a.b.n_seq, a.b.max_q);
-    a.row_blocks = c.row_blocks;
     auto go = [&](auto t, auto d) -> cudaError_t {
         constexpr int T = decltype(t)::value, D = decltype(d)::value;
         if (c.team) {

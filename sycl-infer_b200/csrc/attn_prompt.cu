@@ -369,7 +369,7 @@ template <int T, int D> struct Prompt {
         auto hint_q = [&]() {
             PromptSeg y = x;
             PromptUnit v = u;
-            if (w == 1 && a.vec && advance(y, v)) {
+            if (w == 1 && a.vec && a.group * D * 4 <= 65536 && advance(y, v)) {
                 const int t0 = v.row0 / a.group, t1 = (v.row0 + v.rows - 1) / a.group;
                 for (int i = t0 + lane; i <= t1; i += 32) {
                     const float * q = a.q + (size_t)(v.r.row0 + i) * a.q_stride + (size_t)y.h * a.group * D;
@@ -686,7 +686,7 @@ template <int T, int D> struct Prompt {
                     __threadfence();
                     tile_sync(t);
                     if (tid == 0) {
-                        uint32_t * counter = a.counters + ((size_t)(x.s * a.kv.n_kv + x.h) * a.row_blocks + x.rb) * 2 + t;
+                        uint32_t * counter = a.counters + b0 * 2 + t; // one unit at most starts in a CTA's share and runs on behind it
                         const bool end = atomicAdd(counter, 1u) == (uint32_t)(b1 - b0);
                         if (end) {
                             *counter = 0; // as the next call wants it
@@ -767,8 +767,8 @@ template <int T, int D> __global__ void __launch_bounds__(kPrThreads, 1) attn_pr
     uint8_t * gen = smem_raw + (base - raw);
     constexpr uint32_t HDR = (4 + P::SLOTS) * P::TILE;
     const uint32_t hdr = base + HDR;
-    // header: q_full[2] @0, s_full[2] @16, p_full[2] @32, drain @48, kv_full[6] @64, kv_empty[6] @128, sums @192,
-    // seen groups of eight tiles @256, last[2] @320, tensor memory address @328, fail @332, found share @336
+    // header: q_full[2] @0, s_full[2] @16, p_full[2] @32, drain @48, kv_full[6] @64, kv_empty[6] @128, seen groups of eight
+    // tiles @256, last[2] @320, tensor memory address @328, fail @332, found share @336, sums @352
     P p{a, base, hdr, 0, reinterpret_cast<volatile int *>(gen + HDR + 332), {hdr, hdr + 16, hdr + 32, hdr + 64, hdr + 128, hdr + 48}, {0, 0, 0}};
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     asm volatile("griddepcontrol.launch_dependents;");
@@ -794,12 +794,12 @@ template <int T, int D> __global__ void __launch_bounds__(kPrThreads, 1) attn_pr
     // ---- the CTA's share of the list: units by (sequence, row block, KV head).  The first blocks of the sequences
     // go through shared memory (the tiles' space, not yet in use), then the threads look at a (sequence, row block) each.
     int * first_block = reinterpret_cast<int *>(gen); // [n_seq + 1]
-    volatile int * s_sum = reinterpret_cast<volatile int *>(gen + HDR + 192); // one a warp
-    auto block_scan = [&](int v, int & before) { // sum over the threads below; returns the block's sum
-        int y = v;
+    volatile long long * s_sum = reinterpret_cast<volatile long long *>(gen + HDR + 352); // one a warp
+    auto block_scan = [&](long long v, long long & before) { // sum over the threads below; returns the block's sum
+        long long y = v;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int z = __shfl_up_sync(~0u, y, d);
+            const long long z = __shfl_up_sync(~0u, y, d);
             y += lane >= d ? z : 0;
         }
         __syncthreads();
@@ -807,7 +807,7 @@ template <int T, int D> __global__ void __launch_bounds__(kPrThreads, 1) attn_pr
             s_sum[warp] = y;
         }
         __syncthreads();
-        int all = 0, mine = 0;
+        long long all = 0, mine = 0;
 #pragma unroll
         for (int w = 0; w < kPrThreads / 32; w++) {
             mine += w < warp ? s_sum[w] : 0;
@@ -816,13 +816,14 @@ template <int T, int D> __global__ void __launch_bounds__(kPrThreads, 1) attn_pr
         before = mine + y - v;
         return all;
     };
-    int n_pairs = 0, before;
+    int n_pairs = 0;
+    long long before;
     for (int s0 = 0; s0 < a.b.n_seq; s0 += kPrThreads) {
         const int s = s0 + tid;
         const int v = s < a.b.n_seq ? (seq_rows(a.b, a.kv.page_shift, s).n_run * a.group + kPrRows - 1) / kPrRows : 0;
-        const int all = block_scan(v, before);
+        const int all = (int)block_scan(v, before);
         if (s < a.b.n_seq) {
-            first_block[s] = n_pairs + before;
+            first_block[s] = n_pairs + (int)before;
         }
         n_pairs += all;
     }
@@ -848,12 +849,14 @@ template <int T, int D> __global__ void __launch_bounds__(kPrThreads, 1) attn_pr
         find(pair, s, rb);
         return p.unit(s, rb).k.count + kPrUnitCost;
     };
-    int s_first = 0, rb_first = 0, before_first = 0;
-    const int v_first = cost(tid, s_first, rb_first), all_first = block_scan(v_first, before_first);
-    total = (long long)all_first * a.kv.n_kv;
+    int s_first = 0, rb_first = 0;
+    long long before_first = 0;
+    const int v_first = cost(tid, s_first, rb_first);
+    const long long all_first = block_scan(v_first, before_first);
+    total = all_first * a.kv.n_kv;
     for (int p0 = kPrThreads; p0 < n_pairs; p0 += kPrThreads) {
         int s, rb;
-        total += (long long)block_scan(cost(p0 + tid, s, rb), before) * a.kv.n_kv;
+        total += block_scan(cost(p0 + tid, s, rb), before) * a.kv.n_kv;
     }
     const long long want = (total + a.min_tiles - 1) / a.min_tiles;
     const long long nw = max(1LL, want < gridDim.x ? want : gridDim.x);
@@ -867,21 +870,22 @@ template <int T, int D> __global__ void __launch_bounds__(kPrThreads, 1) attn_pr
     if (work) {
         long long run = 0;
         for (int p0 = 0; p0 < n_pairs; p0 += kPrThreads) {
-            int v = v_first, s = s_first, rb = rb_first, all = all_first;
+            int v = v_first, s = s_first, rb = rb_first;
+            long long all = all_first;
             before = before_first;
             if (p0 > 0) {
                 v = cost(p0 + tid, s, rb);
                 all = block_scan(v, before);
             }
-            const long long b = run + (long long)before * a.kv.n_kv;
+            const long long b = run + before * a.kv.n_kv;
             if (v > 0 && c0 >= b && c0 < b + (long long)v * a.kv.n_kv) {
-                const int in = (int)(c0 - b);
+                const long long in = c0 - b;
                 found[0] = s;
                 found[1] = rb;
-                found[2] = in / v;
-                found[3] = in % v;
+                found[2] = (int)(in / v);
+                found[3] = (int)(in % v);
             }
-            run += (long long)all * a.kv.n_kv;
+            run += all * a.kv.n_kv;
             if (run > c0) {
                 break;
             }
@@ -943,13 +947,10 @@ template <int T, int D> static cudaError_t launch_t(cudaStream_t s, const AttnDe
     return cudaLaunchKernelEx(&cfg, attn_prompt_kernel<T, D>, a);
 }
 
-size_t attn_prompt_units(int n_head, int n_kv, int n_seq, int max_q) { // counters: two tiles a unit
-    return (size_t)n_seq * n_kv * (((size_t)max_q * (n_head / n_kv) + kPrRows - 1) / kPrRows) * 2;
-}
+static_assert(kSMs * 2 <= kAttnCounters, "a counter for every CTA and tile");
 size_t attn_prompt_part_bytes(int head_dim) { return (size_t)kSMs * 4 * pr_part_floats(head_dim) * sizeof(float); }
 
 cudaError_t launch_attn_prompt(cudaStream_t s, AttnDev a) {
-    a.row_blocks = (int)(((long long)a.b.max_q * a.group + kPrRows - 1) / kPrRows);
     a.min_tiles = 2;
     a.vec = !((uintptr_t)a.q & 15) && !((uintptr_t)a.out & 15) && !(a.q_stride & 3) && !(a.out_stride & 3);
     switch (a.kv.type) {

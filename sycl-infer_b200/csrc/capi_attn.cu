@@ -95,12 +95,7 @@ static bool rows_overlap(const float * a, int a_stride, int a_n, const float * b
     return true;
 }
 
-// arrival counters of a call
-static size_t attn_units(int n_head, int n_kv, int n_seq, int max_q) {
-    return (long long)max_q * (n_head / n_kv) <= kDecodeRows ? attn_decode_units(n_head, n_kv, n_seq, max_q)
-                                                             : attn_prompt_units(n_head, n_kv, n_seq, max_q);
-}
-static size_t counter_bytes(size_t units) { return (units * sizeof(uint32_t) + 255) / 256 * 256; }
+constexpr size_t kCounterBytes = kAttnCounters * sizeof(uint32_t);
 
 } // namespace b200q
 
@@ -185,7 +180,7 @@ size_t b200q_attn_scratch_bytes(int n_head, int n_kv, int head_dim, int n_seq, i
     const int mq = max_q < n_tok ? max_q : (n_tok > 0 ? n_tok : 1);
     const size_t parts = (long long)mq * (n_head / n_kv) <= kDecodeRows ? attn_decode_part_bytes(n_head, n_kv, head_dim, n_seq, mq)
                                                                         : attn_prompt_part_bytes(head_dim);
-    return counter_bytes(attn_units(n_head, n_kv, n_seq, mq)) + parts;
+    return kCounterBytes + parts;
 }
 
 int b200q_attn(void * stream, const float * q, int q_stride, int n_head, const b200q_kv_cache * cache,
@@ -208,6 +203,10 @@ int b200q_attn(void * stream, const float * q, int q_stride, int n_head, const b
                   who, n_head, a.kv.n_kv);
         return B200Q_EINVAL;
     }
+    if ((long long)a.b.max_q * (n_head / a.kv.n_kv) > (1 << 30)) {
+        set_error("%s: max_q * n_head / n_kv must not exceed 2^30", who);
+        return B200Q_EUNSUPPORTED;
+    }
     if (a.b.n_tok == 0) {
         return B200Q_OK;
     }
@@ -222,10 +221,10 @@ int b200q_attn(void * stream, const float * q, int q_stride, int n_head, const b
             return B200Q_EINVAL;
         }
         scale = opts->scale;
-        a.window = opts->window;
-        a.n_sink = opts->window ? opts->n_sink : 0;
+        constexpr int far = 1 << 30; // no key is further; keeps the kernels' differences in 32 bits
+        a.window = opts->window < far ? opts->window : far;
+        a.n_sink = opts->window ? (opts->n_sink < far ? opts->n_sink : far) : 0;
     }
-    const size_t units = attn_units(n_head, a.kv.n_kv, a.b.n_seq, a.b.max_q);
     const size_t need = b200q_attn_scratch_bytes(n_head, a.kv.n_kv, D, a.b.n_seq, a.b.n_tok, a.b.max_q);
     if (!scratch || !aligned(scratch, 16) || scratch_bytes < need) {
         set_error("%s: scratch must be 16-byte aligned and hold %zu bytes (got %zu)", who, need, scratch_bytes);
@@ -243,7 +242,7 @@ int b200q_attn(void * stream, const float * q, int q_stride, int n_head, const b
     a.scale_log2 = (float)((double)scale * 1.4426950408889634 * (double)a.kv.k_scale);
     a.v_scale = a.kv.v_scale;
     a.counters = static_cast<uint32_t *>(scratch);
-    a.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + counter_bytes(units));
+    a.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + kCounterBytes);
     if ((long long)a.b.max_q * a.group <= kDecodeRows) {
         B200Q_CUDA_OK(launch_attn_decode((cudaStream_t)stream, a));
     } else {
@@ -276,6 +275,10 @@ int b200q_kv_copy_pages(void * stream, const b200q_kv_cache * layers, int n_laye
     }
     if (n > first.n_pages / 2) {
         set_error("%s: %d pairs of distinct pages do not fit a pool of %d", who, n, first.n_pages);
+        return B200Q_EINVAL;
+    }
+    if ((long long)n * kv_copy_chunks(first) > INT32_MAX) {
+        set_error("%s: too many pages for one call (%d)", who, n);
         return B200Q_EINVAL;
     }
     for (int l0 = 0; l0 < n_layers; l0 += kCopyLayers) {

@@ -32,6 +32,7 @@ cudaError_t launch_rope_append(cudaStream_t s, const double * table, int n_rot, 
                                float * q_out, int q_out_stride, const KvDev & kv, const BatchDev & b);
 cudaError_t launch_kv_copy_pages(cudaStream_t s, const KvDev & c, void * const * pools, int n_pools, const int32_t * src,
                                  const int32_t * dst, int n);
+int kv_copy_chunks(const KvDev & c); // blocks that copy one page
 cudaError_t launch_kv_remap(cudaStream_t s, const int32_t * table, int table_stride, int n_seq, int width,
                             const int32_t * map, int n_pages, int32_t * out, int out_stride);
 
@@ -45,7 +46,7 @@ struct SeqRows {
     int row0;  // first row
     int n_row; // rows the sequence owns
     int n_run; // rows that are computed (at most max_q)
-    int n;     // keys in the cache, the new ones included
+    int n;     // keys in the cache, the new ones included; at most 2^30
 };
 __device__ __forceinline__ SeqRows seq_rows(const BatchDev & b, int page_shift, int s) {
     SeqRows r;
@@ -54,7 +55,7 @@ __device__ __forceinline__ SeqRows seq_rows(const BatchDev & b, int page_shift, 
     const int end = min(max(e, r.row0), b.n_tok);
     r.n_row = end - r.row0;
     r.n_run = min(r.n_row, b.max_q);
-    const long long cap = (long long)b.table_stride << page_shift;
+    const long long cap = min((long long)b.table_stride << page_shift, 1LL << 30); // tile arithmetic stays in 32 bits
     r.n = (int)min((long long)max(n, 0), cap);
     return r;
 }

@@ -73,6 +73,9 @@ static cudaLaunchConfig_t chained(cudaStream_t s, dim3 grid, int threads, cudaLa
     return cfg;
 }
 
+static int64_t page_value_bytes(const KvDev & c) { return (int64_t)c.n_kv * c.head_dim * kv_elem_bytes(c.type) << c.page_shift; }
+int kv_copy_chunks(const KvDev & c) { return (int)((page_value_bytes(c) + kCopyChunk - 1) / kCopyChunk); }
+
 cudaError_t launch_kv_copy_pages(cudaStream_t s, const KvDev & c, void * const * pools, int n_pools, const int32_t * src,
                                  const int32_t * dst, int n) {
     CopyArgs a = {};
@@ -82,9 +85,9 @@ cudaError_t launch_kv_copy_pages(cudaStream_t s, const KvDev & c, void * const *
     a.src = src;
     a.dst = dst;
     a.page_bytes = c.page_bytes;
-    a.bytes = (int64_t)c.n_kv * c.head_dim * kv_elem_bytes(c.type) << c.page_shift;
+    a.bytes = page_value_bytes(c);
     a.n_pages = c.n_pages;
-    a.chunks = (int32_t)((a.bytes + kCopyChunk - 1) / kCopyChunk);
+    a.chunks = kv_copy_chunks(c);
     cudaLaunchAttribute attr[1];
     const cudaLaunchConfig_t cfg = chained(s, dim3((unsigned)n * a.chunks, (unsigned)n_pools), kCopyThreads, attr);
     return cudaLaunchKernelEx(&cfg, copy_pages_kernel, a);

@@ -70,6 +70,8 @@ def test_refused_attention(pkg, capi):
     assert need > 0 and attn(lib, capi, nbytes=need - 1) == 1 and str(need) in lib.last_error()
     for bad in ((4, 3, 64, 1, 1, 1), (4, 2, 80, 1, 1, 1), (0, 1, 64, 1, 1, 1), (4, 2, 64, 0, 1, 1), (4, 2, 64, 1, 1, 0)):
         assert lib.attn_scratch_bytes(*bad) == 0
+    assert attn(lib, capi, b=batch(capi, n_seq=4097)) == 2 and "4096" in lib.last_error()
+    assert attn(lib, capi, b=batch(capi, n_tok=2 ** 30, max_q=2 ** 30)) == 2
     # no rows: nothing to do, nothing launched
     assert attn(lib, capi, b=batch(capi, n_tok=0)) == 0 and append(lib, capi, b=batch(capi, n_tok=0)) == 0
 

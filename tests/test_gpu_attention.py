@@ -1,8 +1,9 @@
 """Rotary append, paged attention and page operators against plain 64-bit forms.
 
 Attention's tolerance, element by element (natural exponent, a = largest scale * sum_d |q_d k_d|):
-a score is off by at most a * (s + (D + 8) 2^-24): s from splitting q into two 16-bit parts (2^-18 for bf16, each
-part half a step of 2^-8; 2^-22 for fp16 parts), the rest from fp32 sums over D products and the two roundings of the
+a score is off by at most a * (s + (D + 8) 2^-24): s from splitting q into 16-bit parts, each of which leaves half a step
+(fp16 2^-11, bf16 2^-8) of what the part before it left: 2^-22 for two fp16 parts (fp16 and e4m3 caches), 2^-24 for the three bf16
+parts of up to 16 query rows a KV head, 2^-16 for the two of more rows; the rest from fp32 sums over D products and the two roundings of the
 scaling; relative weights by twice that (numerator and sum), plus s again for the split of the weights, plus 2^-21
 for ex2.approx (2^-22, numerator and sum), plus fp32 sums over n keys, which run in chains of n / 16 + 32 at most.
 The output is a weighted mean of v, so it is off by at most that times the largest |v| of its head.
@@ -64,6 +65,10 @@ def dense(pool, table, n, page, scale):
     return got.transpose(0, 1)
 
 
+def split_error(dtype, rows):
+    return 2.0 ** -22 if dtype != torch.bfloat16 else (2.0 ** -24 if rows <= 16 else 2.0 ** -16)
+
+
 def attn_ref(cache, batch, q, lens, first, window, sinks, scale):
     """(out, tolerance) in 64 bits, one row and head at a time over the keys that it sees."""
     n_tok, qd = q.shape
@@ -71,7 +76,7 @@ def attn_ref(cache, batch, q, lens, first, window, sinks, scale):
     group = qd // dim // cache.n_kv
     out = torch.zeros(n_tok, qd, dtype=torch.float64, device="cuda")
     tol = torch.zeros_like(out)
-    split = 2.0 ** -18 if cache.k.dtype == torch.bfloat16 else 2.0 ** -22
+    split = split_error(cache.k.dtype, group * batch.max_q)
     for s, (n_q, n) in enumerate(lens):
         if n == 0:
             continue
@@ -175,6 +180,105 @@ def test_large_scores_and_values(be, pkg):
         q.mul_(30.0)
         cache.v.mul_(1000.0)
         check_attn(be, pkg, cache, batch, q, lens, first)
+
+
+@pytest.mark.parametrize("lens", [[(1, 300), (1, 77)], [(60, 60), (3, 200)]])
+@pytest.mark.parametrize("typ", ["f16", "e4m3"])
+def test_unaligned_rows(be, pkg, typ, lens):
+    """Rows of q and out that start off 16 bytes and lie an odd number of values apart."""
+    cache, batch, q, first = make_step(pkg, typ, lens, 2, 3, 64, 16)
+    wide = torch.randn(q.shape[0], q.shape[1] + 3, device="cuda")
+    view = wide[:, 1:1 + q.shape[1]]
+    out = torch.zeros(q.shape[0], q.shape[1] + 5, device="cuda")[:, 3:3 + q.shape[1]]
+    be.attn(view, out, cache, batch, pkg.alloc_attn_scratch(6, cache, batch))
+    ref, tol = attn_ref(cache, batch, view, lens, first, 0, 0, 64 ** -0.5)
+    n = first[-1]
+    assert bool(((out[:n].double() - ref[:n]).abs() <= tol[:n]).all()) and bool((out[n:] == 0).all())
+
+
+@pytest.mark.parametrize("group,lens", [(1, [(40, 70), (20, 20)]), (17, [(1, 90), (2, 33)]), (40, [(1, 200)]), (300, [(3, 50)]), (7, [(19, 400), (37, 37)])])
+def test_prompt_groups(be, pkg, group, lens):
+    """Head groups that do not divide the row tiles, larger than one among them."""
+    cache, batch, q, first = make_step(pkg, "f16", lens, 1, group, 64, 16)
+    check_attn(be, pkg, cache, batch, q, lens, first)
+
+
+def test_rows_beyond_max_q_are_left(be, pkg):
+    for n_q, max_q in ((5, 2), (60, 40)):
+        lens = [(n_q, 100)]
+        cache, batch, q, first = make_step(pkg, "f16", lens, 1, 4, 64, 16)
+        short = pkg.kv_batch(batch.page_table, batch.q_start, batch.kv_len, batch.n_tok, max_q)
+        out = torch.full(q.shape, 5.0, device="cuda")
+        be.attn(q, out, cache, short, pkg.alloc_attn_scratch(4, cache, short))
+        ref, tol = attn_ref(cache, short, q, lens, first, 0, 0, 64 ** -0.5)
+        assert bool(((out[:max_q].double() - ref[:max_q]).abs() <= tol[:max_q]).all()) and bool((out[max_q:] == 5).all())
+
+
+def test_a_window_without_end(be, pkg):
+    """The largest window and sink count are no window at all."""
+    for lens in ([(1, 700)], [(50, 300)]):
+        cache, batch, q, first = make_step(pkg, "bf16", lens, 1, 4, 64, 16)
+        check_attn(be, pkg, cache, batch, q, lens, first, 2 ** 31 - 1, 2 ** 31 - 1)
+
+
+def test_one_scratch_for_calls_of_all_shapes(be, pkg):
+    """Decode and prompt steps of few and of many sequences take turns on one scratch: none finds another's leavings."""
+    steps = []
+    for lens, kv, group, dim, typ in ([(1, 5000)], 2, 4, 64, "bf16"), ([(1, 40 + i) for i in range(150)], 2, 4, 128, "f16"), \
+            ([(300, 900), (40, 2000)], 2, 8, 128, "f16"), ([(3, 3000)] * 3, 1, 5, 128, "bf16"), ([(100, 100)] * 5, 2, 4, 64, "e4m3"):
+        cache, batch, q, first = make_step(pkg, typ, lens, kv, group, dim, 16)
+        ref, tol = attn_ref(cache, batch, q, lens, first, 0, 0, dim ** -0.5)
+        need = pkg.load_lib().attn_scratch_bytes(kv * group, kv, dim, batch.n_seq, batch.n_tok, batch.max_q)
+        steps.append((cache, batch, q, first[-1], ref, tol, need))
+    scratch = torch.zeros(max(s[-1] for s in steps), dtype=torch.uint8, device="cuda")
+    for turn in range(4):
+        for cache, batch, q, n, ref, tol, _ in (steps if turn % 2 else steps[::-1]):
+            out = torch.empty(q.shape, device="cuda")
+            be.attn(q, out, cache, batch, scratch)
+            assert bool(((out[:n].double() - ref[:n]).abs() <= tol[:n]).all())
+    assert bool((scratch[:8192] == 0).all())
+
+
+def test_two_streams_at_once(be, pkg):
+    """Calls on two streams, each with a scratch of its own, do not disturb each other."""
+    backs, runs = [pkg.make_cuda_backend(0, torch.cuda.Stream()) for _ in range(2)], []
+    for b, lens in zip(backs, ([(1, 9000), (1, 30)], [(130, 700), (9, 9)])):
+        cache, batch, q, first = make_step(pkg, "f16", lens, 2, 4, 64, 16)
+        ref, tol = attn_ref(cache, batch, q, lens, first, 0, 0, 64 ** -0.5)
+        runs.append((b, cache, batch, q, first[-1], ref, tol, pkg.alloc_attn_scratch(8, cache, batch), [torch.zeros(q.shape, device="cuda") for _ in range(12)]))
+    torch.cuda.synchronize()
+    for i in range(12):
+        for b, cache, batch, q, n, ref, tol, scratch, outs in runs:
+            b.attn(q, outs[i], cache, batch, scratch)
+    torch.cuda.synchronize()
+    for b, cache, batch, q, n, ref, tol, scratch, outs in runs:
+        for out in outs:
+            assert bool(((out[:n].double() - ref[:n]).abs() <= tol[:n]).all())
+
+
+def test_a_pool_beyond_4_gb(be, pkg):
+    """Pages whose byte offsets pass 32 bits: append, both attentions and the page copy reach them."""
+    n_pages, page, dim = 9, 16, 64
+    mem = torch.empty(2, n_pages, 1 << 28, dtype=torch.bfloat16, device="cuda")  # 512 MB from page to page
+    k, v = (m[:, :2 * page * dim].view(n_pages, 2, page, dim) for m in mem)
+    k.zero_()
+    v.zero_()
+    cache = pkg.kv_cache(k, v)
+    table = torch.tensor([[8, 0, 7]], dtype=torch.int32).cuda()
+    n = 40
+    batch = pkg.kv_batch(table, torch.tensor([0, n], dtype=torch.int32).cuda(), torch.tensor([n], dtype=torch.int32).cuda(), n, n)
+    x = torch.randn(n, 8 * dim, device="cuda")
+    q, kn, vn = x.split([4 * dim, 2 * dim, 2 * dim], 1)
+    be.rope_append(None, None, kn, vn, None, cache, batch)
+    for i in range(n):
+        p, at = int(table[0, i // page]), i % page
+        assert torch.equal(k[p, :, at].flatten(), kn[i].bfloat16()) and torch.equal(v[p, :, at].flatten(), vn[i].bfloat16())
+    lens = [(n, n)]
+    check_attn(be, pkg, cache, batch, q, lens, [0, n])
+    one = pkg.kv_batch(table, torch.tensor([0, 1], dtype=torch.int32).cuda(), batch.kv_len, 1, 1)
+    check_attn(be, pkg, cache, one, q[:1], [(1, n)], [0, 1])
+    be.kv_copy_pages([cache], torch.tensor([8, 0], dtype=torch.int32).cuda(), torch.tensor([1, 6], dtype=torch.int32).cuda())
+    assert torch.equal(k[1], k[8]) and torch.equal(v[6], v[0])
 
 
 def test_results_do_not_depend_on_arrival(be, pkg):
@@ -443,7 +547,6 @@ def test_pool_prompt_fork_decode_compact(be, pkg, typ):
     turns, factor = turns_ref(dim, 1e4)
     book = {}  # sequence -> per layer (k, v) as stored
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
-    split = 2.0 ** -18 if typ == "bf16" else 2.0 ** -22
 
     def step(sids, new):
         moves = [m for s, n in zip(sids, new) for m in pool.extend(s, n)]
@@ -482,6 +585,7 @@ def test_pool_prompt_fork_decode_compact(be, pkg, typ):
                     w = torch.softmax(xk.sum(-1) / math.sqrt(dim), -1)
                     want = torch.einsum("hj,hjd->hd", w, V[:, :m]).flatten()
                     a = float(xk.abs().sum(-1).max()) / math.sqrt(dim)
+                    split = split_error(TYPES[typ], group * batch.max_q)
                     lim = float(V[:, :m].abs().max()) * (2 * a * (split + (dim + 8) * 2.0 ** -24) + split + 2.0 ** -21 + 2 * (m / 16 + 32) * 2.0 ** -24)
                     assert bool(((out[row].double() - want).abs() <= lim).all())
                     row += 1
