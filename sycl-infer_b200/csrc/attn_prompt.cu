@@ -582,38 +582,57 @@ template <int T, int D> struct Prompt {
                         return (valid >> (c / 16)) & 1 ? bits : 0u;
                     };
                     float top = -INFINITY;
-                    auto look = [&](int c, uint64_t (&v)[8]) {
-                        if (!whole) { // masked scores go back: the second reading needs no masks
-                            const uint32_t bits = seen(c);
-#pragma unroll
-                            for (int i = 0; i < 8; i++) {
-                                v[i] = pair2((bits >> (2 * i)) & 1 ? first2(v[i]) : -INFINITY,
-                                             (bits >> (2 * i + 1)) & 1 ? second2(v[i]) : -INFINITY);
+                    // On a border, most groups of 16 keys are still seen by all rows of the warp or by none: only the others
+                    // take masks, and their masked scores go back, so that the second reading needs none.  The two
+                    // kinds of tile have code of their own: the tests would cost whole tiles 5 %.
+                    uint32_t some = 0xFFu, mixed = 0;
+                    auto look = [&](int c, uint64_t (&v)[8], auto border) {
+                        if constexpr (decltype(border)::value) {
+                            if (!((some >> (c / 16)) & 1)) {
+                                return;
                             }
-                            tmem_st16(s_cols + c, v);
+                            if ((mixed >> (c / 16)) & 1) {
+                                const uint32_t bits = seen(c);
+#pragma unroll
+                                for (int i = 0; i < 8; i++) {
+                                    v[i] = pair2((bits >> (2 * i)) & 1 ? first2(v[i]) : -INFINITY,
+                                                 (bits >> (2 * i + 1)) & 1 ? second2(v[i]) : -INFINITY);
+                                }
+                                tmem_st16(s_cols + c, v);
+                            }
                         }
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             top = fmaxf(top, fmaxf(first2(v[i]), second2(v[i])));
                         }
                     };
-                    {
+                    auto maximum = [&](auto border) {
                         uint64_t v[2][8];
                         tmem_ld16(s_cols, v[0]);
 #pragma unroll 1
                         for (int c = 0; c < kPrKeys; c += 32) {
                             tmem_ld_wait();
                             tmem_ld16(s_cols + c + 16, v[1]);
-                            look(c, v[0]);
+                            look(c, v[0], border);
                             tmem_ld_wait();
                             if (c + 32 < kPrKeys) {
                                 tmem_ld16(s_cols + c + 32, v[0]);
                             }
-                            look(c + 16, v[1]);
+                            look(c + 16, v[1], border);
                         }
-                        if (!whole) {
-                            tmem_st_wait();
+                    };
+                    if (whole) {
+                        maximum(std::false_type{});
+                    } else {
+                        some = 0;
+#pragma unroll 1
+                        for (int g = 0; g < kPrKeys / 16; g++) {
+                            const uint32_t bits = seen(16 * g);
+                            some |= __any_sync(~0u, bits != 0) ? 1u << g : 0u;
+                            mixed |= __all_sync(~0u, bits == 0xFFFFu) ? 0u : 1u << g;
                         }
+                        maximum(std::true_type{});
+                        tmem_st_wait();
                     }
                     const float mn = fmaxf(m, top * cq);
                     const float f_new = m == mn ? 1.0f : exp2_fast(m - mn);
@@ -621,8 +640,19 @@ template <int T, int D> struct Prompt {
                     m = mn;
                     uint64_t sum = 0, sum1 = 0;
                     const uint64_t cc = pair2(cq, cq), oo = pair2(off, off);
-                    auto weigh = [&](int c, const uint64_t (&v)[8]) { // p of 16 keys takes the place of their s
+                    auto weigh = [&](int c, const uint64_t (&v)[8], auto border) { // p of 16 keys takes the place of their s
                         uint32_t hi[8], lo[8];
+                        if constexpr (decltype(border)::value) {
+                            if (!((some >> (c / 16)) & 1)) {
+#pragma unroll
+                                for (int i = 0; i < 8; i++) {
+                                    hi[i] = 0;
+                                }
+                                tmem_st8(s_cols + c, hi);
+                                tmem_st8(s_cols + c + 8, hi);
+                                return;
+                            }
+                        }
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             const uint64_t e = fma2(v[i], cc, oo);
@@ -641,20 +671,25 @@ template <int T, int D> struct Prompt {
                         tmem_st8(s_cols + c, hi);
                         tmem_st8(s_cols + c + 8, lo);
                     };
-                    {
+                    auto weights = [&](auto border) {
                         uint64_t v[2][8];
                         tmem_ld16(s_cols, v[0]);
 #pragma unroll 1
                         for (int c = 0; c < kPrKeys; c += 32) {
                             tmem_ld_wait();
                             tmem_ld16(s_cols + c + 16, v[1]);
-                            weigh(c, v[0]);
+                            weigh(c, v[0], border);
                             tmem_ld_wait();
                             if (c + 32 < kPrKeys) {
                                 tmem_ld16(s_cols + c + 32, v[0]);
                             }
-                            weigh(c + 16, v[1]);
+                            weigh(c + 16, v[1], border);
                         }
+                    };
+                    if (whole) {
+                        weights(std::false_type{});
+                    } else {
+                        weights(std::true_type{});
                     }
                     sum = add2(sum, sum1);
                     l = fmaf(l, f_new, first2(sum) + second2(sum));
