@@ -18,11 +18,12 @@
 //   Tensor memory: s of both tiles (128 columns each; p's two parts take the place of s as it is consumed), p v of both.
 // * Every wait is bounded; when one runs out the status word is set and all roles run to their end without waiting.
 //
-// B200: 512 tokens after 32001 keys f16 615 us alone, 725 us in a run of them at the power limit: 1.10 and 0.93 PFLOP/s of tensor
-// work (the two parts), 66 % of the measured burst and 67 % of the sustained bf16 rate.  A step of two tiles takes
+// B200: 512 tokens after 32001 keys f16 591 us alone, 710 us in a run of them at the power limit: 1.14 and 0.95 PFLOP/s of tensor
+// work (the two parts), 69 % of the measured burst and 69 % of the sustained bf16 rate.  A step of two tiles takes
 // 7600 clocks of which the tensor pipe works 54 %; the softmax of a tile takes 4500, two thirds of it loads from tensor memory
-// that nothing hides (330 clocks each).  Wider loads (64 columns) spill and lose: 672 us.  Prompts of 2048 tokens bf16
-// 128 us and short windows are bound by what a unit costs beside its tiles: q in, rows out, the first scores (about 9 us a unit).
+// that nothing hides (330 clocks each while products run).  Wider loads (64 columns) spill and lose: 672 us.  Prompts of 2048
+// tokens bf16 (122 us) and short windows are bound by what a unit costs beside its tiles: q in, rows out, the first scores (about 9 us).
+// bf16 keys widened to fp16 by the producers, for 22 bits there too, made the prompt of 2048 tokens 270 us: not taken.
 #include "async.cuh"
 #include "attn.cuh"
 

@@ -281,6 +281,19 @@ def test_a_pool_beyond_4_gb(be, pkg):
     assert torch.equal(k[1], k[8]) and torch.equal(v[6], v[0])
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("k_size,v_size", [(1.0, 1e-7), (1.0, 3e9), (2e6, 1.0), (1e-9, 1e-20), (1e20, 1e30), (1.0, 0.0)])
+def test_bf16_prompts_of_any_magnitude(be, pkg, dim, k_size, v_size):
+    """Keys and values far outside fp16's range, unequal from page to page: bf16 has it."""
+    lens = [(60, 400), (33, 33)]
+    cache, batch, q, first = make_step(pkg, "bf16", lens, 2, 4, dim, 16)
+    cache.k.mul_(k_size)
+    cache.v.mul_(v_size)
+    cache.v[1::3].mul_(0.001)  # and unequal from page to page
+    q.mul_(1.0 / k_size)
+    check_attn(be, pkg, cache, batch, q, lens, first)
+
+
 def test_results_do_not_depend_on_arrival(be, pkg):
     lens = [(1, 20000), (1, 3000), (1, 50)]
     cache, batch, q, first = make_step(pkg, "bf16", lens, 2, 4, 64, 64)
