@@ -428,8 +428,8 @@ int b200q_attn(void * stream, const float * q, int q_stride, int n_head, const b
 
 /* Copies page src[i] to page dst[i] of every layer, K and V, for i < n, in one launch per 64 layers: the last
  * page of a forked sequence, the moves that compact a pool.  The layers' caches differ in k and v only.
- * dst entries must be distinct and none may also be a src entry of another pair (the copies run at the same
- * time).  A pair with an entry outside [0, n_pages) is left out and b200q_device_status reports
+ * dst entries must be distinct and none may also be a src entry (the copies run at the same time); one page may
+ * be the src of many.  A pair with an entry outside [0, n_pages) is left out and b200q_device_status reports
  * B200Q_EINVAL. */
 int b200q_kv_copy_pages(void * stream, const b200q_kv_cache * layers /*host*/, int n_layers, const int32_t * src,
                         const int32_t * dst, int n);

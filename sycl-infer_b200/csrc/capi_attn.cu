@@ -273,8 +273,8 @@ int b200q_kv_copy_pages(void * stream, const b200q_kv_cache * layers, int n_laye
     if (n == 0) {
         return B200Q_OK;
     }
-    if (n > first.n_pages / 2) {
-        set_error("%s: %d pairs of distinct pages do not fit a pool of %d", who, n, first.n_pages);
+    if (n >= first.n_pages) { // one source may have many copies, but the copies are distinct and none is a source
+        set_error("%s: %d copies do not fit a pool of %d pages", who, n, first.n_pages);
         return B200Q_EINVAL;
     }
     if ((long long)n * kv_copy_chunks(first) > INT32_MAX) {

@@ -94,7 +94,7 @@ def test_refused_page_operators(pkg, capi):
     two = (capi.KvCache * 2)(cache(capi), cache(capi))
     assert lib.kv_copy_pages(None, two, 0, P, P, 1) == 1 and lib.kv_copy_pages(None, two, 2, None, P, 1) == 1
     assert lib.kv_copy_pages(None, two, 2, P, P, -1) == 1 and lib.kv_copy_pages(None, two, 2, None, None, 0) == 0
-    assert lib.kv_copy_pages(None, two, 2, P, P, 5) == 1  # ten distinct pages of a pool of eight
+    assert lib.kv_copy_pages(None, two, 2, P, P, 8) == 1  # eight copies and a source in a pool of eight
     for kw in (dict(n_pages=9), dict(type=1), dict(n_kv=1), dict(page_stride=4096)):
         assert lib.kv_copy_pages(None, (capi.KvCache * 2)(cache(capi), cache(capi, **kw)), 2, P, P, 1) == 1, kw
     ok = (None, P, 8, 2, 8, 2 * P, 4, 3 * P, 8)

@@ -520,6 +520,16 @@ def test_copy_pages(be, pkg, typ, layers, n_kv, page, dim, moves):
     assert be.device_status() == 0
 
 
+def test_one_page_copied_to_all_others(be, pkg):
+    """A sequence forked into as many as the pool holds: one source, every other page a copy."""
+    pool = torch.randn(9, 2, 16, 64, device="cuda").to(torch.bfloat16)
+    cache = pkg.kv_cache(pool, pool.clone())
+    dst = torch.tensor([p for p in range(9) if p != 4], dtype=torch.int32).cuda()
+    be.kv_copy_pages([cache], torch.full_like(dst, 4), dst)
+    be.synchronize()
+    assert all(torch.equal(pool[p], pool[4]) and torch.equal(cache.v[p], cache.v[4]) for p in range(9)) and be.device_status() == 0
+
+
 def test_copy_pages_bad_pairs_are_left_out(be, pkg):
     pool = torch.randn(8, 2, 16, 64, device="cuda").to(torch.bfloat16)
     cache = pkg.kv_cache(pool, pool.clone())
