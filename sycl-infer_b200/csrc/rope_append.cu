@@ -16,7 +16,7 @@ namespace b200q {
 
 __device__ int g_append_status = 0;
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;
 constexpr int kMaxRot = 128;
 
 __global__ void rope_table_kernel(const __grid_constant__ b200q_rope r, double * __restrict__ table) {
@@ -60,7 +60,9 @@ struct AppendArgs {
 // VEC = 4: an item is eight values of a head as two float4: in the rotated part four pairs (half layout: the second float4
 // lies half a rotation behind the first; interleaved: next to it), behind it, and in v, eight neighbours.  VEC = 1: an item is
 // one pair, for any alignment and any even n_rot.
-constexpr int kRopeBatch = 2; // items of a thread in flight (1, 2, 4: 25.6, 24.5, 25.8 us for 2048 tokens)
+// Many small blocks hide each other's chain best.  2048 tokens / 900 in 48 chunks: 256 threads with two items each in flight
+// 24.1 / 11.0 us, 128 threads with two 23.1 / 10.3, with one (ten blocks an SM) 23.1 / 9.1.
+constexpr int kRopeBatch = 1; // items of a thread in flight
 
 template <int T, int VEC> struct RopeItem {
     float u[VEC], v[VEC]; // values d0.. and d1..
@@ -69,7 +71,7 @@ template <int T, int VEC> struct RopeItem {
     int h;
 };
 
-template <int T, int VEC> __global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const __grid_constant__ AppendArgs a) {
+template <int T, int VEC> __global__ void __launch_bounds__(kRopeThreads, 10) rope_append_kernel(const __grid_constant__ AppendArgs a) {
     __shared__ float2 cs[kMaxRot / 2];
     __shared__ int s_seq;
     asm volatile("griddepcontrol.launch_dependents;");
