@@ -764,7 +764,8 @@ template <int T, int D> struct Prompt {
                     }
                 }
                 if (write) {
-                    // through the tile's q space, whose products are done, so that rows leave whole; the warp's own 32 rows
+                    // through the tile's q space, whose products are done, so that rows leave whole; a warp takes back the 32
+                    // rows that it put there
                     const float inv = l > 0.0f || isnan(l) ? a.v_scale / l : 0.0f; // no visible key: zeros
                     const uint64_t ii = pair2(inv, inv);
                     const uint32_t stage = q_addr(t, 0) + (uint32_t)warp_row * D * 4;
@@ -791,7 +792,9 @@ template <int T, int D> struct Prompt {
                             }
                         }
                     }
-                    __syncwarp(); // the space takes the next unit's q
+                    // The space takes the next unit's q, whose swizzled blocks of any warp lie over the rows of several: none
+                    // before all four have sent theirs.
+                    tile_sync(t);
                 }
             }
             tile_n += (uint32_t)n;

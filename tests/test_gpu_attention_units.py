@@ -1,0 +1,155 @@
+"""Attention over so many units that a block of the grid (or a warp of it) goes from one to the next: the borders
+between units, where shared memory, barriers and tensor memory change hands.  Everything is held to a 64-bit form at
+test_gpu_attention.py's tolerance, and repeated calls to the same bits.
+"""
+import pytest
+import torch
+
+from test_gpu_attention import TYPES, split_error
+
+SMS = 148  # blocks of the prompt kernel's grid
+
+
+# ---- what the kernels share out, by the rules at the head of their files --------------------------------------
+
+def key_tiles(pos_first, n, keys, window, sinks):
+    """Tiles of `keys` keys that some row sees, the first of them at position pos_first, of n keys."""
+    oldest = min(max(0, pos_first - window + 1) if window else 0, n)
+    lo = oldest // keys
+    return max(1, min(-(-min(sinks, n) // keys), lo) + -(-n // keys) - lo)
+
+
+def prompt_units(lens, n_kv, group, window=0, sinks=0):
+    """Tiles of every unit (256 rows of a KV head) in the list's order."""
+    got = []
+    for q, n in lens:
+        for r0 in range(0, q * group, 256):
+            r1 = min(q * group, r0 + 256) - 1
+            got += [key_tiles(n - q + r0 // group, min(n, max(0, n - q + r1 // group + 1)), 128, window, sinks)] * n_kv
+    return got
+
+
+def units_of_blocks(tiles):
+    """How many units each block of the prompt kernel works on: equal shares of the list of tiles, three more a unit."""
+    total = sum(t + 3 for t in tiles)
+    blocks = min(SMS, -(-total // 2))
+    each, more = divmod(total, blocks)
+    got = []
+    for b in range(blocks):
+        lo = b * each + min(b, more)
+        hi = lo + each + (b < more)
+        at = n = 0
+        for t in tiles:
+            n += min(hi, at + 3 + t) > max(lo, at + 3)
+            at += 3 + t
+        got.append(n)
+    return got
+
+
+# ---- a step and its 64-bit form ---------------------------------------------------------------------------------
+
+def ragged_step(pkg, typ, lens, n_kv, group, dim, page, seed, window=0, sinks=0, spare=2, q_scale=1.0):
+    """(cache, batch, q, first row of each sequence, keys, values): what no row sees is NaN, in the pages too."""
+    gen = torch.Generator().manual_seed(seed)
+    scales = (0.0625, 0.03125) if typ == "e4m3" else (1.0, 1.0)
+    first = [0]
+    for q, _ in lens:
+        first.append(first[-1] + q)
+    held = [-(-n // page) for _, n in lens]
+    order = torch.randperm(sum(held) + 2, generator=gen).to(torch.int32)
+    pools = [torch.full((sum(held) + 2, n_kv, page, dim), float("nan")) for _ in range(2)]
+    table, at, dense = torch.full((len(lens), max(1, *held) + 1), -1, dtype=torch.int32), 0, []
+    for s, (q, n) in enumerate(lens):
+        j = torch.arange(held[s] * page)
+        oldest = max(0, n - q - window + 1) if window and q else 0
+        hidden = (j >= n) | ((j < oldest) & (j >= sinks))
+        both = []
+        for pool, scale in zip(pools, scales):
+            x = torch.randn(n_kv, len(j), dim, generator=gen) / scale
+            x = x.to(TYPES[typ]).float()
+            x[:, hidden] = float("nan")
+            pool[order[at:at + held[s]].long()] = x.view(n_kv, held[s], page, dim).transpose(0, 1)
+            both.append((x[:, :n] * scale).cuda().double())
+        dense.append(both)
+        table[s, :held[s]] = order[at:at + held[s]]
+        at += held[s]
+    n_tok = first[-1] + spare
+    q = (q_scale * torch.randn(n_tok, n_kv * group * dim, generator=gen)).cuda()
+    cache = pkg.kv_cache(pools[0].to(TYPES[typ]).cuda(), pools[1].to(TYPES[typ]).cuda(), *scales)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    batch = pkg.kv_batch(table.cuda(), i32(first), i32([n for _, n in lens]), n_tok, max(1, *(q for q, _ in lens)))
+    return cache, batch, q, first, dense
+
+
+def reference(cache, batch, q, lens, first, dense, window=0, sinks=0, scale=None):
+    """(out, tolerance) in 64 bits; the tolerance is derived at the head of test_gpu_attention.py."""
+    dim, kv = cache.head_dim, cache.n_kv
+    group = q.shape[1] // dim // kv
+    scale = scale or dim ** -0.5
+    split = split_error(cache.k.dtype, group * batch.max_q)
+    out, tol = (torch.zeros(first[-1], kv, group, dim, dtype=torch.float64, device="cuda") for _ in range(2))
+    for s, (n_q, n) in enumerate(lens):
+        if not n_q or not n:
+            continue
+        rows = slice(first[s], first[s] + n_q)
+        x = q[rows].double().view(n_q, kv, group, dim)
+        pos, j = torch.arange(n - n_q, n, device="cuda")[:, None], torch.arange(n, device="cuda")[None]
+        seen = j <= pos
+        if window:
+            seen &= (j > pos - window) | (j < sinks)
+        used = seen.any(0)
+        k, v = (t.where(used[None, :, None], torch.zeros_like(t)) for t in dense[s])
+        m = seen[:, None, None, :]
+        w = torch.softmax(torch.einsum("thgd,hjd->thgj", x, k).mul(scale).masked_fill(~m, float("-inf")), -1)
+        w = w.masked_fill(~m, 0.0)  # rows that see nothing: zeros
+        out[rows] = torch.einsum("thgj,hjd->thgd", w, v)
+        a = torch.einsum("thgd,hjd->thgj", x.abs(), k.abs()).masked_fill(~m, 0.0).amax((1, 2, 3)) * scale
+        rel = 2 * a * (split + (dim + 8) * 2.0 ** -24) + split + 2.0 ** -21 + 2 * (n / 16 + 32) * 2.0 ** -24
+        top = v.abs().amax(2)[None].where(seen[:, None, :], torch.zeros((), dtype=torch.float64, device="cuda")).amax(2)
+        tol[rows] = (rel[:, None] * top)[:, :, None, None]
+    return out.flatten(1), tol.flatten(1)
+
+
+def check(be, pkg, cache, batch, q, lens, first, dense, window=0, sinks=0, scale=None, repeats=1):
+    ref, tol = reference(cache, batch, q, lens, first, dense, window, sinks, scale)
+    scratch = pkg.alloc_attn_scratch(q.shape[1] // cache.head_dim, cache, batch)
+    outs = torch.full((repeats, *q.shape), 77.0, device="cuda")
+    for out in outs:
+        be.attn(q, out, cache, batch, scratch, scale=scale, window=window, n_sink=sinks)
+    be.synchronize()
+    n = first[-1]
+    assert bool((outs[:, n:] == 77).all()) and be.device_status() == 0
+    err = (outs[0, :n].double() - ref).abs()
+    assert not bool(err.isnan().any())
+    worst = float((err / tol.clamp(min=1e-30)).max())
+    assert worst <= 1.0, f"{worst} of the tolerance"
+    assert all(torch.equal(out, outs[0]) for out in outs[1:])
+
+
+# ---- prompts ----------------------------------------------------------------------------------------------------
+
+# (tokens, cache) of the sequences, KV heads, group, window, sinks.  Row blocks end with 1, 20, 33 and 96 live rows (whole
+# warps of a tile without any), with more than one tile, and full; units of one tile and of several follow each other.
+def _prompts():
+    one = [(1, 40), (20, 20), (33, 300), (96, 97), (257, 257), (17, 700), (276, 280), (128, 128), (289, 400), (352, 352)] * 8
+    five = [(1, 130), (4, 4), (7, 260), (19, 19), (52, 52), (58, 190), (0, 50), (26, 513)] * 12
+    far = [(1, 900), (33, 1000), (20, 20), (129, 640), (5, 3), (97, 97)] * 14
+    return {"heads of their own": (one, 8, 1, 0, 0), "groups of five": (five, 8, 5, 0, 0), "window": (far, 8, 4, 70, 4)}
+
+
+@pytest.mark.parametrize("name", list(_prompts()))
+def test_prompt_steps_have_borders(name):
+    lens, n_kv, group, window, sinks = _prompts()[name]
+    per = units_of_blocks(prompt_units(lens, n_kv, group, window, sinks))
+    assert len(per) == SMS and min(per) >= 3, per
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("typ", ["bf16", "f16", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("name", list(_prompts()))
+def test_prompt_blocks_go_from_unit_to_unit(be, pkg, name, typ, dim):
+    lens, n_kv, group, window, sinks = _prompts()[name]
+    step = ragged_step(pkg, typ, lens, n_kv, group, dim, 16, seed=dim, window=window, sinks=sinks)
+    cache, batch, q, first, dense = step
+    check(be, pkg, cache, batch, q, lens, first, dense, window, sinks, repeats=50)
