@@ -18,7 +18,7 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int * status) {
+__device__ __forceinline__ bool mbar_wait_some(uint32_t bar, uint32_t parity) { // false: kSpinCycles went by
     long long t0 = 0;
     for (uint32_t n = 0;; n++) {
         uint32_t ok;
@@ -33,8 +33,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int * s
         if (n == 64) {
             t0 = clock64();
         } else if (n > 64 && clock64() - t0 > kSpinCycles) {
-            break;
+            return false;
         }
+    }
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int * status) {
+    if (mbar_wait_some(bar, parity)) {
+        return true;
     }
     atomicExch(status, B200Q_ETIMEOUT);
     return false;

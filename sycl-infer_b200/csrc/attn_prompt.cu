@@ -16,7 +16,8 @@
 //   products; warps 9-11 bring K and V into shared memory in the 128-byte swizzled form (16-bit caches by asynchronous
 //   copies, e4m3 widened to fp16 on the way), rows that nobody sees as zeros.
 //   Tensor memory: s of both tiles (128 columns each; p's two parts take the place of s as it is consumed), p v of both.
-// * Every wait is bounded; when one runs out the status word is set and all roles run to their end without waiting.
+// * Every wait is bounded, by a time in which the CTA's products have not moved on; when one runs out the status word is
+//   set and all roles run to their end without waiting.
 //
 // B200: 512 tokens after 32001 keys f16 591 us alone, 710 us in a run of them at the power limit: 1.14 and 0.95 PFLOP/s of tensor
 // work (the two parts), 69 % of the measured burst and 69 % of the sustained bf16 rate.  A step of two tiles takes
@@ -185,20 +186,31 @@ template <int T, int D> struct Prompt {
     uint32_t hdr;
     uint32_t tmem;
     volatile int * fail;
+    volatile int * progress; // the product warp's last item
     PromptBars bars;
     PromptShare share;
 
     __device__ __forceinline__ uint32_t q_addr(int tile, int part) const { return base + (tile * 2 + part) * TILE; }
     __device__ __forceinline__ uint32_t slot_addr(int slot) const { return base + (4 + slot) * TILE; }
 
-    // a bounded wait; after one has run out nobody waits any more
+    // A bounded wait; after one has run out nobody waits any more.  While products are issued the time starts anew: the second
+    // tile's warps wait for as long as the CTA works on units without one, which may be most of a long call.
     __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity) const {
         if (*fail) {
             return;
         }
-        if (!mbar_wait(bar, parity, &g_attn_prompt_status)) {
-            *fail = 1;
+        if (mbar_wait_some(bar, parity)) {
+            return;
         }
+        int at;
+        do {
+            at = *progress;
+            if (mbar_wait_some(bar, parity)) {
+                return;
+            }
+        } while (*progress != at);
+        atomicExch(&g_attn_prompt_status, B200Q_ETIMEOUT);
+        *fail = 1;
     }
 
     __device__ __forceinline__ PromptUnit unit(int s, int rb) const {
@@ -281,6 +293,7 @@ template <int T, int D> struct Prompt {
             release(item);
             for (int j = 0; j < n; j++) {
                 const uint32_t iv = item + 2 * j + 1, ik = iv + 1;
+                *progress = (int)iv;
                 for (int t = 0; t < tiles; t++) {
                     wait(bars.p_full + 8 * t, (p_par >> t) & 1);
                     p_par ^= 1u << t;
@@ -813,8 +826,9 @@ template <int T, int D> __global__ void __launch_bounds__(kPrThreads, 1) attn_pr
     constexpr uint32_t HDR = (4 + P::SLOTS) * P::TILE;
     const uint32_t hdr = base + HDR;
     // header: q_full[2] @0, s_full[2] @16, p_full[2] @32, drain @48, kv_full[6] @64, kv_empty[6] @128, seen groups of eight
-    // tiles @256, last[2] @320, tensor memory address @328, fail @332, found share @336, sums @352
-    P p{a, base, hdr, 0, reinterpret_cast<volatile int *>(gen + HDR + 332), {hdr, hdr + 16, hdr + 32, hdr + 64, hdr + 128, hdr + 48}, {0, 0, 0}};
+    // tiles @256, last[2] @320, tensor memory address @328, fail @332, found share @336, sums @352,
+    // progress @448
+    P p{a, base, hdr, 0, reinterpret_cast<volatile int *>(gen + HDR + 332), reinterpret_cast<volatile int *>(gen + HDR + 448), {hdr, hdr + 16, hdr + 32, hdr + 64, hdr + 128, hdr + 48}, {0, 0, 0}};
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 0) {
@@ -829,6 +843,7 @@ template <int T, int D> __global__ void __launch_bounds__(kPrThreads, 1) attn_pr
         }
         mbar_init(p.bars.drain, 1);
         *p.fail = 0;
+        *p.progress = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 8) {

@@ -153,3 +153,32 @@ def test_prompt_blocks_go_from_unit_to_unit(be, pkg, name, typ, dim):
     step = ragged_step(pkg, typ, lens, n_kv, group, dim, 16, seed=dim, window=window, sinks=sinks)
     cache, batch, q, first, dense = step
     check(be, pkg, cache, batch, q, lens, first, dense, window, sinks, repeats=50)
+
+
+@pytest.mark.gpu
+def test_a_wait_lasts_as_long_as_the_block_works(be, pkg):
+    """The second row tile's warps have nothing to do in units of up to 128 rows.  4095 sequences of such units over a
+    million keys each, then one of 136 rows: they wait for seconds while all is well, and must not give up.  All
+    tables name one page, so key j is key j mod 128."""
+    n_seq, n_kv, group, dim, page, n, n_q = 4096, 4, 17, 64, 128, 1 << 20, 8
+    gen = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(1, n_kv, page, dim, generator=gen).to(torch.float16).cuda() for _ in range(2))
+    first = torch.arange(n_seq + 1, dtype=torch.int32)
+    first[-1] += n_q - 1
+    n_tok = n_seq + n_q - 1
+    batch = pkg.kv_batch(torch.zeros(n_seq, n // page, dtype=torch.int32, device="cuda"), first.cuda(),
+                         torch.full((n_seq,), n, dtype=torch.int32, device="cuda"), n_tok, n_q)
+    cache = pkg.kv_cache(k, v)
+    q = torch.randn(n_tok, n_kv * group * dim, generator=gen).cuda()
+    out = torch.full(q.shape, 77.0, device="cuda")
+    be.attn(q, out, cache, batch, pkg.alloc_attn_scratch(n_kv * group, cache, batch))
+    be.synchronize()
+    assert be.device_status() == 0
+    for t, pos in [(0, n - 1), (2000, n - 1)] + [(n_seq - 1 + i, n - n_q + i) for i in range(n_q)]:
+        x = q[t].double().view(n_kv, group, dim)
+        s = torch.einsum("hgd,hjd->hgj", x, k[0].double()) / 8
+        often = (n // page - (torch.arange(page, device="cuda") > pos % page).double()).log()
+        want = torch.einsum("hgj,hjd->hgd", torch.softmax(s + often, -1), v[0].double()).flatten()
+        a = float(torch.einsum("hgd,hjd->hgj", x.abs(), k[0].double().abs()).max()) / 8
+        rel = 2 * a * (2.0 ** -22 + (dim + 8) * 2.0 ** -24) + 2.0 ** -22 + 2.0 ** -21 + 2 * (n / 16 + 32) * 2.0 ** -24
+        assert float((out[t].double() - want).abs().max()) <= rel * float(v.abs().max())
