@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
                           (((unsigned long long)ps.h << a.kv.page_shift) + (k0 & ((1 << a.kv.page_shift) - 1))) * ROWB;
                 } else {
                     seen = 0;
-                    atomicExch(&g_attn_status, B200Q_EINVAL);
+                    note_bad_page(&g_attn_status);
                 }
             }
         }

@@ -378,7 +378,7 @@ template <int T, int D> struct Prompt {
                         }
                     } else {
                         seen = 0;
-                        atomicExch(&g_attn_prompt_status, B200Q_EINVAL);
+                        note_bad_page(&g_attn_prompt_status);
                     }
                 }
             }

@@ -60,6 +60,9 @@ __device__ __forceinline__ SeqRows seq_rows(const BatchDev & b, int page_shift, 
     return r;
 }
 
+// A page id outside the pool: the rest of the call is right.  Never in place of a wait that ran out, after which nothing is.
+__device__ __forceinline__ void note_bad_page(int * status) { atomicCAS(status, 0, B200Q_EINVAL); }
+
 template <int T> struct KvElem;
 template <> struct KvElem<kF16> {
     static constexpr int BYTES = 2;

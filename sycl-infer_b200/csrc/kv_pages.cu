@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
     const int s = a.src[i], d = a.dst[i];
     if (s < 0 || s >= a.n_pages || d < 0 || d >= a.n_pages) {
         if (threadIdx.x == 0) {
-            atomicExch(&g_pages_status, B200Q_EINVAL);
+            note_bad_page(&g_pages_status);
         }
         return;
     }

@@ -152,7 +152,7 @@ template <int T, int VEC> __global__ void __launch_bounds__(kRopeThreads, 10) ro
         if (page < 0 || page >= a.kv.n_pages) {
             page = -1;
             if (tid == 0 && blockIdx.y == 0) {
-                atomicExch(&g_append_status, B200Q_EINVAL);
+                note_bad_page(&g_append_status);
             }
         }
     }
