@@ -681,11 +681,19 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
                 p[NT * OV * 32 + x * 16 + 8 + g] = l[x];
             }
         };
-        auto take = [&](const float * p) { // joins another part to the thread's
+        // Joins another part to the thread's; parts in the scratch are other SMs' and come from L2.
+        auto take = [&](const float * p, auto in_scratch) {
+            auto value = [&](int i) {
+                if constexpr (decltype(in_scratch)::value) {
+                    return __ldcg(p + i);
+                } else {
+                    return p[i];
+                }
+            };
             float fa[RX], fb[RX];
 #pragma unroll
             for (int x = 0; x < RX; x++) {
-                const float m2 = p[NT * OV * 32 + x * 16 + g], l2 = p[NT * OV * 32 + x * 16 + 8 + g];
+                const float m2 = value(NT * OV * 32 + x * 16 + g), l2 = value(NT * OV * 32 + x * 16 + 8 + g);
                 const float mn = fmaxf(m[x], m2);
                 fa[x] = m[x] == mn ? 1.0f : exp2_fast(m[x] - mn);
                 fb[x] = m2 == mn ? 1.0f : exp2_fast(m2 - mn);
@@ -695,7 +703,7 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
 #pragma unroll
             for (int j = 0; j < NT * OV; j++) {
                 const int x = H8 ? 0 : (j >> 1) & 1;
-                v[j] = v[j] * fa[x] + p[j * 32 + lane] * fb[x];
+                v[j] = v[j] * fa[x] + value(j * 32 + lane) * fb[x];
             }
         };
         // The team's first warp ends with all: halves of the team put their parts where the warp that takes them has
@@ -709,7 +717,7 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
                     }
                     __syncthreads();
                     if (warp < half) {
-                        take(join + (2 * half == TEAM ? warp : warp + half) * PART);
+                        take(join + (2 * half == TEAM ? warp : warp + half) * PART, std::false_type{});
                     }
                 }
             }
@@ -748,6 +756,7 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
                     }
                 }
                 write = __shfl_sync(~0u, last, 0);
+                __syncwarp(); // what lane 0's fence made visible, for all lanes: the shuffle orders no memory
             }
             if constexpr (TEAM > 1) {
                 __syncthreads();
@@ -764,7 +773,7 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
                     v[j] = 0.0f;
                 }
                 for (int b = b0 + w_first; b <= b1; b += TEAM) {
-                    take(slot(b, b == b0));
+                    take(slot(b, b == b0), std::true_type{});
                 }
                 join_team();
             }

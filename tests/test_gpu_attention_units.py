@@ -182,3 +182,58 @@ def test_a_wait_lasts_as_long_as_the_block_works(be, pkg):
         a = float(torch.einsum("hgd,hjd->hgj", x.abs(), k[0].double().abs()).max()) / 8
         rel = 2 * a * (2.0 ** -22 + (dim + 8) * 2.0 ** -24) + 2.0 ** -22 + 2.0 ** -21 + 2 * (n / 16 + 32) * 2.0 ** -24
         assert float((out[t].double() - want).abs().max()) <= rel * float(v.abs().max())
+
+
+# ---- few rows, many units ---------------------------------------------------------------------------------------
+
+# (tokens, cache) of the sequences, KV heads, group, window, sinks: empty slots, sequences without rows and rows before the
+# first position among them, units of one tile and units that several warps share.
+def _decodes():
+    none = [(0, 77), (1, 0), (0, 0), (2, 1)]
+    one = ([(1, 1 + 37 * i % 611) for i in range(60)] + none) * 8 + [(1, 9000)]
+    some = ([(1 + i % 3, 3 + 53 * i % 700) for i in range(60)] + none) * 8 + [(3, 7000)]
+    return {"one row": (one, 8, 4, 0, 0), "up to 15 rows": (some, 8, 5, 0, 0), "window": (some, 8, 4, 90, 5)}
+
+
+@pytest.mark.parametrize("name", list(_decodes()))
+def test_decode_steps_have_borders(name):
+    """At most 148 x 3 x 4 warps share the units: two and more for each; and the longest unit alone is more than a warp's share."""
+    lens, n_kv, group, window, sinks = _decodes()[name]
+    for keys in (16, 32, 64):  # of a tile, by type and head size
+        tiles = [key_tiles(n - q, n, keys, window, sinks) for q, n in lens if q]
+        assert len(tiles) * n_kv >= 2 * SMS * 3 * 4
+        assert window or max(tiles) > sum(tiles) * n_kv / (SMS * 2 * 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("typ", ["bf16", "f16", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("name", list(_decodes()))
+def test_decode_warps_go_from_unit_to_unit(be, pkg, name, typ, dim):
+    lens, n_kv, group, window, sinks = _decodes()[name]
+    step = ragged_step(pkg, typ, lens, n_kv, group, dim, 16, seed=dim, window=window, sinks=sinks)
+    cache, batch, q, first, dense = step
+    check(be, pkg, cache, batch, q, lens, first, dense, window, sinks, repeats=20)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("typ,low", [("bf16", False), ("f16", False), ("e4m3", False), ("bf16", True), ("f16", True), ("e4m3", True)])
+@pytest.mark.parametrize("rows", [1, 3, 5])
+def test_no_part_of_the_weights_is_lost(be, pkg, typ, low, rows):
+    """Few keys and scores near zero: the tolerance is at its smallest, and weights rounded to one 16-bit part, computed
+    here in 64 bits, are outside it.  low: many units, few without it; 5 rows x 4 heads go to the prompt kernel."""
+    lens = [(rows, rows + 1 + i % 7) for i in range(40 if low else 8)]
+    step = ragged_step(pkg, typ, lens, 2, 4, 64, 16, seed=rows)
+    cache, batch, q, first, dense = step
+    check(be, pkg, cache, batch, q, lens, first, dense, scale=0.004)
+    ref, tol = reference(cache, batch, q, lens, first, dense, scale=0.004)
+    beyond = 0.0
+    for s, (n_q, n) in enumerate(lens):
+        x = q[first[s]:first[s] + n_q].double().view(n_q, 2, 4, 64)
+        m = torch.arange(n, device="cuda")[None] <= torch.arange(n - n_q, n, device="cuda")[:, None]
+        z = torch.einsum("thgd,hjd->thgj", x, dense[s][0]).mul(0.004).masked_fill(~m[:, None, None], float("-inf"))
+        p = torch.exp(z - z.amax(-1, keepdim=True))
+        one = p.to(torch.bfloat16 if typ == "bf16" else torch.float16).double()
+        out = torch.einsum("thgj,hjd->thgd", one / p.sum(-1, keepdim=True), dense[s][1]).flatten(1)
+        beyond = max(beyond, float(((out - ref[first[s]:first[s] + n_q]).abs() / tol[first[s]:first[s] + n_q].clamp(min=1e-30)).max()))
+    assert beyond > 2.0
