@@ -132,6 +132,8 @@ class attn_call:
 class _Seq:
     pages: list = field(default_factory=list)  # page ids in order, -1 = given back (behind the window)
     length: int = 0                            # tokens
+    gone: dict = field(default_factory=dict)   # place of a page given back -> shortest length that does without it
+    widest: int = 0                            # window for which pages were given back
 
 
 class KvPool:
@@ -216,26 +218,28 @@ class KvPool:
             if p >= 0:
                 self.refs[p] += 1
         new = self.new()
-        self._seqs[new] = _Seq(list(q.pages), q.length)
+        self._seqs[new] = _Seq(list(q.pages), q.length, dict(q.gone), q.widest)
         return new
 
     def truncate(self, sid, length):
-        """Forgets the tokens from `length` on (drafts that were not accepted)."""
+        """Forgets the tokens from `length` on (drafts that were not accepted).  Refused, with nothing changed, when the
+        window of the next token would reach a page that trim() has given back: truncate first, then trim."""
         q = self._seq(sid)
         if not 0 <= length <= q.length:
             raise ValueError("KvPool: a length within the sequence")
         keep = -(-length // self.page_size)
-        if any(p < 0 for p in q.pages[keep - 1:keep]):
-            raise ValueError("KvPool: the new last page has been given back")
-        for p in q.pages[keep:]:
-            if p >= 0:
-                self._drop(p)
+        first = max(0, (length - q.widest + 1) // self.page_size)  # of the pages that any such window reaches
+        if any(q.gone.get(i, 0) > length for i in range(first, keep)):
+            raise ValueError(f"KvPool: from token {length} on the window reaches pages that have been given back")
+        for i in range(keep, len(q.pages)):
+            if q.gone.pop(i, None) is None:
+                self._drop(q.pages[i])
         del q.pages[keep:]
         q.length = length
 
     def trim(self, sid, window, n_sink=0):
         """Gives back the pages that no coming token of a sliding window sees: those wholly behind the window of
-        the next token, but for the first n_sink tokens'."""
+        the next token, but for the first n_sink tokens'.  Drafts that may be refused: truncate() comes before trim()."""
         if window < 1 or n_sink < 0:
             raise ValueError("KvPool: window >= 1, n_sink >= 0")
         q = self._seq(sid)
@@ -244,6 +248,8 @@ class KvPool:
             if p >= 0 and (i + 1) * self.page_size <= oldest and i * self.page_size >= n_sink:
                 self._drop(p)
                 q.pages[i] = -1
+                q.gone[i] = (i + 1) * self.page_size + window - 1
+                q.widest = max(q.widest, window)
 
     def free(self, sid):
         q = self._seq(sid)
