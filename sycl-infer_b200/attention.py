@@ -85,12 +85,17 @@ class rope_t:
 
 def alloc_attn_scratch(n_head, cache, batch):
     """Caller-owned scratch of `cuda_backend.attn`: one serves every layer and step of one stream (how much a call needs
-    depends on its shape: take the largest, attn says when it is too small).  Calls that may overlap must not
+    depends on its shape: take the largest, attn says when it is too small).  It is zeroed when the call returns, for a
+    backend on any stream (but for an allocation that is captured: its graph zeroes it).  Calls that may overlap must not
     share it."""
     n = load_lib().attn_scratch_bytes(n_head, cache.n_kv, cache.head_dim, batch.n_seq, batch.n_tok, batch.max_q)
     if n == 0:
         raise ValueError(f"alloc_attn_scratch: unsupported shape ({n_head} heads over {cache.n_kv}, head_dim {cache.head_dim})")
-    return torch.zeros(n, dtype=torch.uint8, device=cache.device)
+    scratch = torch.zeros(n, dtype=torch.uint8, device=cache.device)
+    with torch.cuda.device(cache.device):
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream().synchronize()
+    return scratch
 
 
 @dataclass

@@ -237,3 +237,35 @@ def test_no_part_of_the_weights_is_lost(be, pkg, typ, low, rows):
         out = torch.einsum("thgj,hjd->thgd", one / p.sum(-1, keepdim=True), dense[s][1]).flatten(1)
         beyond = max(beyond, float(((out - ref[first[s]:first[s] + n_q]).abs() / tol[first[s]:first[s] + n_q].clamp(min=1e-30)).max()))
     assert beyond > 2.0
+
+
+# ---- a backend with a stream of its own --------------------------------------------------------------------------
+
+@pytest.mark.gpu
+def test_a_scratch_is_ready_for_any_stream(be, pkg):
+    """The scratch is zeroed on the caller's stream; the first call on a backend's own stream finds it zeroed, however far
+    behind the caller's stream is."""
+    lens = [(1, 9000), (1, 30)]
+    cache, batch, q, first, dense = ragged_step(pkg, "f16", lens, 2, 4, 64, 16, seed=1)
+    ref, tol = reference(cache, batch, q, lens, first, dense)
+    own = pkg.make_cuda_backend(0, torch.cuda.Stream())
+    first_call = pkg.alloc_attn_scratch(8, cache, batch)
+    out = torch.empty(q.shape, device="cuda")
+    torch.cuda.synchronize()
+    own.attn(q, out, cache, batch, first_call)  # a kernel's first launch may wait for the device
+    torch.cuda.synchronize()
+    out.fill_(77.0)
+    nbytes = first_call.nbytes
+    del first_call
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    used = torch.full((nbytes,), 255, dtype=torch.uint8, device="cuda")  # what the allocator hands out again
+    torch.cuda.synchronize()
+    at = used.data_ptr()
+    del used
+    torch.cuda._sleep(200_000_000)  # a tenth of a second
+    scratch = pkg.alloc_attn_scratch(8, cache, batch)
+    assert scratch.data_ptr() == at
+    own.attn(q, out, cache, batch, scratch)
+    torch.cuda.synchronize()
+    assert bool(((out[:2].double() - ref).abs() <= tol).all())
