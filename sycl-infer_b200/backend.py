@@ -238,7 +238,8 @@ class cuda_backend:
     def rope_table(self, rope):
         """Fills rope.table (n_rot / 2 frequencies in turns a position and the factor, 64 bits); once per model."""
         if rope.table is None:
-            rope.table = torch.empty(max(0, rope.c.n_rot) // 2 + 1, dtype=torch.float64, device=self.device)
+            with torch.cuda.stream(self._stream):  # memory of the stream that writes it (None: the current one)
+                rope.table = torch.empty(max(0, rope.c.n_rot) // 2 + 1, dtype=torch.float64, device=self.device)
         self._here(rope.table, *([rope.freq_factors] if rope.freq_factors is not None else []))
         self._call(self.lib.rope_table, rope.ref, rope.table.data_ptr())
         return rope.table

@@ -269,3 +269,19 @@ def test_a_scratch_is_ready_for_any_stream(be, pkg):
     own.attn(q, out, cache, batch, scratch)
     torch.cuda.synchronize()
     assert bool(((out[:2].double() - ref).abs() <= tol).all())
+
+
+@pytest.mark.gpu
+def test_a_rotary_table_is_its_streams_own(be, pkg):
+    """The table is written on the backend's stream: its memory must not be some that the caller's stream has yet to write to."""
+    want = be.rope_table(pkg.rope_t(128, base=1e6)).clone()
+    own = pkg.make_cuda_backend(0, torch.cuda.Stream())
+    held = [torch.empty(65, dtype=torch.float64, device="cuda") for _ in range(4200)]  # whatever the allocator has of this size
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
+    held[-1].fill_(7.0)
+    held.pop()
+    rope = pkg.rope_t(128, base=1e6)
+    own.rope_table(rope)
+    torch.cuda.synchronize()
+    assert torch.equal(rope.table, want)
