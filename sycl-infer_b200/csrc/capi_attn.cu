@@ -50,8 +50,9 @@ static int check_cache(const char * who, const b200q_kv_cache * c, KvDev & d) {
 }
 
 static int check_batch(const char * who, const b200q_kv_batch * b, BatchDev & d) {
-    if (!b || !b->page_table || !b->q_start || !b->kv_len) {
-        set_error("%s: the batch's page_table, q_start and kv_len must be non-null", who);
+    if (!b || !b->page_table || !b->q_start || !b->kv_len || !aligned(b->page_table, 4) || !aligned(b->q_start, 4) ||
+        !aligned(b->kv_len, 4)) {
+        set_error("%s: the batch's page_table, q_start and kv_len must be non-null and 4-byte aligned", who);
         return B200Q_EINVAL;
     }
     if (b->n_seq < 1 || b->n_tok < 0 || b->max_q < 1 || b->table_stride < 1) {
@@ -108,8 +109,8 @@ int b200q_rope_table(void * stream, const b200q_rope * rope, double * table) {
     if (rc != B200Q_OK) {
         return rc;
     }
-    if (!table || !aligned(table, 8)) {
-        set_error("b200q_rope_table: table must be non-null and 8-byte aligned");
+    if (!table || !aligned(table, 8) || !aligned(rope->freq_factors, 4)) {
+        set_error("b200q_rope_table: table must be non-null and 8-byte aligned, freq_factors 4-byte aligned");
         return B200Q_EINVAL;
     }
     if (!(rope->base > 1.0f) || std::isinf(rope->base) || !(rope->freq_scale > 0.0f) || !(rope->freq_scale <= 1.0f) ||
@@ -142,8 +143,8 @@ int b200q_rope_append(void * stream, const double * table, const b200q_rope * ro
         set_error("%s: n_rot must not exceed head_dim, the table must be 8-byte aligned (n_rot=%d)", who, rope->n_rot);
         return B200Q_EINVAL;
     }
-    if ((!q && !k) || (!k) != (!v) || (q && !q_out)) {
-        set_error("%s: q with q_out, or k with v, or both must be non-null", who);
+    if ((!q && !k) || (!k) != (!v) || (q && !q_out) || !aligned(q, 4) || !aligned(k, 4) || !aligned(v, 4) || (q && !aligned(q_out, 4))) {
+        set_error("%s: q with q_out, or k with v, or both must be non-null, and 4-byte aligned", who);
         return B200Q_EINVAL;
     }
     const int kd = kv.n_kv * kv.head_dim;
@@ -195,7 +196,7 @@ int b200q_attn(void * stream, const float * q, int q_stride, int n_head, const b
     }
     const int D = a.kv.head_dim;
     if (!q || !out || !aligned(q, 4) || !aligned(out, 4)) {
-        set_error("%s: q and out must be non-null", who);
+        set_error("%s: q and out must be non-null and 4-byte aligned", who);
         return B200Q_EINVAL;
     }
     if (n_head < 1 || n_head > 8192 || n_head % a.kv.n_kv || q_stride < n_head * D || out_stride < n_head * D) {
@@ -254,8 +255,8 @@ int b200q_attn(void * stream, const float * q, int q_stride, int n_head, const b
 int b200q_kv_copy_pages(void * stream, const b200q_kv_cache * layers, int n_layers, const int32_t * src, const int32_t * dst,
                         int n) {
     const char * who = "b200q_kv_copy_pages";
-    if (!layers || n_layers < 1 || n < 0 || (n > 0 && (!src || !dst))) {
-        set_error("%s: layers, src and dst must be non-null, n_layers >= 1, n >= 0", who);
+    if (!layers || n_layers < 1 || n < 0 || (n > 0 && (!src || !dst || !aligned(src, 4) || !aligned(dst, 4)))) {
+        set_error("%s: layers, src and dst must be non-null (src and dst 4-byte aligned), n_layers >= 1, n >= 0", who);
         return B200Q_EINVAL;
     }
     KvDev first, d;
@@ -296,8 +297,9 @@ int b200q_kv_copy_pages(void * stream, const b200q_kv_cache * layers, int n_laye
 int b200q_kv_remap(void * stream, const int32_t * table, int table_stride, int n_seq, int width, const int32_t * map, int n_pages,
                    int32_t * out, int out_stride) {
     const char * who = "b200q_kv_remap";
-    if (!table || !map || !out || n_seq < 1 || width < 1 || n_pages < 1 || table_stride < width || out_stride < width) {
-        set_error("%s: table, map and out must be non-null, n_seq, width and n_pages >= 1, strides >= width", who);
+    if (!table || !map || !out || !aligned(table, 4) || !aligned(map, 4) || !aligned(out, 4) || n_seq < 1 || width < 1 || n_pages < 1 ||
+        table_stride < width || out_stride < width) {
+        set_error("%s: table, map and out must be non-null and 4-byte aligned, n_seq, width and n_pages >= 1, strides >= width", who);
         return B200Q_EINVAL;
     }
     if (!(table == out && table_stride == out_stride) &&

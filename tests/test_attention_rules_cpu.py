@@ -1,5 +1,6 @@
 """The attention side without a GPU, continued: what a status word holds, the pool's window, pointers that kernels
 would follow to an unaligned address."""
+import ctypes as C
 import os
 import random
 import re
@@ -70,3 +71,40 @@ def test_pages_in_the_window_survive_trim_and_truncate(pkg, seed):
             else:
                 pool.truncate(s, n)
         assert all(pool.pages(s)[i] >= 0 for i in _needed(pool.length(s), window, sinks, size))
+
+
+def test_unaligned_pointers_are_refused(pkg):
+    """No entry point hands a kernel an address that its loads and stores would fault on."""
+    from sycl_infer_b200 import capi
+    lib, P = pkg.load_lib(), 1 << 20
+
+    def cache():
+        return capi.KvCache(P, 2 * P, 30, 8, 16, 2, 64, 2 * 16 * 64, 1.0, 1.0)
+
+    def batch(**kw):
+        d = dict(page_table=P, q_start=P, kv_len=P, table_stride=4, n_seq=2, n_tok=3, max_q=2)
+        return C.byref(capi.KvBatch(**{**d, **kw}))
+
+    def rope(**kw):
+        return C.byref(capi.Rope(**{**dict(n_rot=64, base=1e4, freq_scale=1.0, attn_factor=1.0, beta_fast=32.0, beta_slow=1.0), **kw}))
+
+    def append(b=None, q=4 * P, k=6 * P, v=7 * P, out=8 * P):
+        return lib.rope_append(None, P, rope(), q, 512, 4, k, 128, v, 128, out, 256, C.byref(cache()), b or batch())
+
+    def attn(b=None, q=4 * P, out=8 * P):
+        return lib.attn(None, q, 256, 4, C.byref(cache()), b or batch(), None, out, 256, 16 * P, 1 << 40)
+
+    for off in (1, 2, 3):
+        for name in ("page_table", "q_start", "kv_len"):
+            assert append(batch(**{name: P + off})) == 1 and attn(batch(**{name: P + off})) == 1, name
+            assert "aligned" in lib.last_error()
+        for name, base in (("q", 4 * P), ("k", 6 * P), ("v", 7 * P), ("out", 8 * P)):
+            assert append(**{name: base + off}) == 1, name
+        assert attn(q=4 * P + off) == 1 and attn(out=8 * P + off) == 1
+        assert lib.rope_table(None, rope(freq_factors=P + off), P) == 1
+        arr = (capi.KvCache * 1)(cache())
+        assert lib.kv_copy_pages(None, arr, 1, P + off, P, 1) == 1 and lib.kv_copy_pages(None, arr, 1, P, P + off, 1) == 1
+        for i in (1, 5, 7):
+            a = [None, P, 8, 2, 8, 2 * P, 4, 3 * P, 8]
+            a[i] += off
+            assert lib.kv_remap(*a) == 1, i
