@@ -22,6 +22,13 @@ def _int32(t, what, dims):
         raise ValueError(f"{what}: a {dims}-dimensional int32 CUDA tensor with unit stride is expected")
 
 
+def _int(value, what):
+    """An int32 of the C structs, of which ctypes would silently keep the low bits; what is too small the library refuses."""
+    if not -2 ** 31 <= value < 2 ** 31:
+        raise ValueError(f"{what}: {value} does not fit 32 bits")
+    return int(value)
+
+
 class kv_cache:
     """K and V of one layer: tensors [n_pages][n_kv][page_size][head_dim] of float16, bfloat16 or
     float8_e4m3fn; the pages may lie further apart than they are long (a view of a pool that other layers
@@ -63,7 +70,8 @@ class kv_batch:
         if stride != page_table.shape[1]:
             raise ValueError("kv_batch: page_table must be contiguous")
         self.page_table, self.q_start, self.kv_len = page_table, q_start, kv_len
-        self.device, self.n_seq, self.n_tok, self.max_q = kv_len.device, n_seq, int(n_tok), int(max_q)
+        self.device, self.n_seq = kv_len.device, n_seq
+        self.n_tok, self.max_q = _int(n_tok, "kv_batch: n_tok"), _int(max_q, "kv_batch: max_q")
         self.c = KvBatch(page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), stride, n_seq, self.n_tok, self.max_q)
         self.ref = C.byref(self.c)
 
@@ -77,8 +85,8 @@ class rope_t:
                                          not freq_factors.is_contiguous() or freq_factors.numel() != n_rot // 2):
             raise ValueError("rope_t: freq_factors is a contiguous float32 CUDA tensor of n_rot / 2 values")
         self.freq_factors = freq_factors
-        self.c = Rope(n_rot, 1 if interleaved else 0, base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow, n_ctx_orig,
-                      freq_factors.data_ptr() if freq_factors is not None else None)
+        self.c = Rope(_int(n_rot, "rope_t: n_rot"), 1 if interleaved else 0, base, freq_scale, ext_factor, attn_factor, beta_fast,
+                      beta_slow, _int(n_ctx_orig, "rope_t: n_ctx_orig"), freq_factors.data_ptr() if freq_factors is not None else None)
         self.ref = C.byref(self.c)
         self.table = None  # n_rot / 2 + 1 doubles
 

@@ -16,7 +16,7 @@ from typing import Optional
 
 import torch
 
-from .attention import _int32
+from .attention import _int, _int32
 from .capi import MAX_SEGS, AttnOpts, Seg, load_lib
 
 
@@ -66,6 +66,8 @@ def _rows(t, what, index, n_rows, width=None):
     if len(shape) != 2 or shape[0] != n_rows or (width is not None and shape[1] != width) or (stride[1] != 1 and n_rows):
         raise ValueError(f"{what}: {n_rows} rows" + (f" of {width} values" if width is not None else "") +
                          f" with unit stride are expected (got shape {tuple(shape)}, strides {stride})")
+    if stride[0] > 0x7FFFFFFF and n_rows > 1:
+        raise ValueError(f"{what}: rows {stride[0]} values apart, 2^31 - 1 at most are supported")
     return t.data_ptr(), stride[0] if n_rows > 1 else shape[1], shape[1]
 
 
@@ -284,11 +286,12 @@ class cuda_backend:
             raise ValueError("attn: the rows of q are not a multiple of head_dim")
         if not scratch.is_contiguous():
             raise ValueError("attn: the scratch must be contiguous")
-        if scale is not None and not scale > 0:
-            raise ValueError("attn: scale must be above 0 (None: 1 / sqrt(head_dim))")
+        scale = 0.0 if scale is None else C.c_float(scale).value or -1.0  # the C side's 0 stands for None
+        if not scale >= 0:
+            raise ValueError("attn: scale must be above 0 in 32 bits (None: 1 / sqrt(head_dim))")
+        opts = AttnOpts(scale, _int(window, "attn: window"), _int(n_sink, "attn: n_sink"))
         if n == 0:
             return
-        opts = AttnOpts(scale or 0.0, window, n_sink)
         self._call(self._attn, qp, qs, n_head, cache.ref, batch.ref, C.byref(opts), op, os_, scratch.data_ptr(), scratch.nbytes)
 
     def kv_copy_pages(self, caches, src, dst):

@@ -108,3 +108,27 @@ def test_unaligned_pointers_are_refused(pkg):
             a = [None, P, 8, 2, 8, 2 * P, 4, 3 * P, 8]
             a[i] += off
             assert lib.kv_remap(*a) == 1, i
+
+
+def test_counts_beyond_32_bits_are_refused(pkg):
+    """Not cut to their low 32 bits."""
+    import torch
+    from sycl_infer_b200.backend import _rows
+    for kw in (dict(n_rot=2 ** 32 + 64), dict(n_rot=64, n_ctx_orig=2 ** 32 + 4096)):
+        with pytest.raises(ValueError):
+            pkg.rope_t(**kw)
+
+    class view:  # rows that far apart take more memory than there is
+        dtype, shape = torch.float32, (2, 256)
+        get_device, data_ptr = (lambda self: 0), (lambda self: 1 << 20)
+
+        def __init__(self, apart):
+            self.apart = apart
+
+        def stride(self):
+            return self.apart, 1
+
+    assert _rows(view(2 ** 31 - 1), "q", 0, 2) == (1 << 20, 2 ** 31 - 1, 256)
+    for apart in (2 ** 31, 2 ** 32 + 256):
+        with pytest.raises(ValueError, match="apart"):
+            _rows(view(apart), "q", 0, 2)

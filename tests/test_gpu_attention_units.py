@@ -285,3 +285,22 @@ def test_a_rotary_table_is_its_streams_own(be, pkg):
     own.rope_table(rope)
     torch.cuda.synchronize()
     assert torch.equal(rope.table, want)
+
+
+@pytest.mark.gpu
+def test_arguments_beyond_32_bits_are_refused(be, pkg):
+    cache, batch, q, first, dense = ragged_step(pkg, "f16", [(1, 40)], 1, 1, 64, 16, seed=1)
+    scratch, out = pkg.alloc_attn_scratch(1, cache, batch), torch.empty(q.shape, device="cuda")
+    for kw in (dict(window=2 ** 32 + 5), dict(window=2 ** 31), dict(window=5, n_sink=2 ** 32), dict(scale=1e-46), dict(scale=0.0),
+               dict(scale=float("nan")), dict(scale=-1.0)):
+        with pytest.raises(ValueError):
+            be.attn(q, out, cache, batch, scratch, **kw)
+    for kw in (dict(window=-1), dict(window=5, n_sink=-1)):
+        with pytest.raises(pkg.B200QError):
+            be.attn(q, out, cache, batch, scratch, **kw)
+    for n_tok, max_q in ((2 ** 32 + 1, 1), (1, 2 ** 32 + 1)):
+        with pytest.raises(ValueError):
+            pkg.kv_batch(batch.page_table, batch.q_start, batch.kv_len, n_tok, max_q)
+    be.attn(q, out, cache, batch, scratch, window=2 ** 31 - 1, n_sink=2 ** 31 - 1, scale=1e-40)
+    be.synchronize()
+    assert torch.allclose(out[0].double(), dense[0][1][0].mean(0), atol=1e-5, rtol=0)  # no score counts
