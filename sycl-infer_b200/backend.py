@@ -286,12 +286,11 @@ class cuda_backend:
             raise ValueError("attn: the rows of q are not a multiple of head_dim")
         if not scratch.is_contiguous():
             raise ValueError("attn: the scratch must be contiguous")
-        scale = 0.0 if scale is None else C.c_float(scale).value or -1.0  # the C side's 0 stands for None
-        if not scale >= 0:
+        if scale is not None and not C.c_float(scale).value > 0:  # the C side's 0 stands for None
             raise ValueError("attn: scale must be above 0 in 32 bits (None: 1 / sqrt(head_dim))")
-        opts = AttnOpts(scale, _int(window, "attn: window"), _int(n_sink, "attn: n_sink"))
         if n == 0:
             return
+        opts = AttnOpts(scale or 0.0, window and _int(window, "attn: window"), n_sink and _int(n_sink, "attn: n_sink"))
         self._call(self._attn, qp, qs, n_head, cache.ref, batch.ref, C.byref(opts), op, os_, scratch.data_ptr(), scratch.nbytes)
 
     def kv_copy_pages(self, caches, src, dst):
