@@ -36,6 +36,7 @@
 namespace b200q {
 
 __device__ int g_attn_status = 0;
+static std::atomic<bool> g_launched{false}; // nothing to read before
 
 constexpr int kDecStageBytes = 8192; // K and V halves of one tile
 constexpr int kDecTeam = 8;          // warps of a CTA that work on one piece
@@ -866,6 +867,7 @@ size_t attn_decode_part_bytes(int n_head, int n_kv, int head_dim, int n_seq, int
 }
 
 cudaError_t launch_attn_decode(cudaStream_t s, const AttnDev & a) {
+    g_launched = true;
     const DecodeCut c = decode_cut(a.kv.type, a.group, a.kv.n_kv, a.b.n_seq, a.b.max_q);
     auto go = [&](auto t, auto d) -> cudaError_t {
         constexpr int T = decltype(t)::value, D = decltype(d)::value;
@@ -889,6 +891,10 @@ cudaError_t launch_attn_decode(cudaStream_t s, const AttnDev & a) {
 }
 
 cudaError_t read_attn_status(int * status, bool clear) {
+    if (!g_launched) {
+        *status = 0;
+        return cudaSuccess;
+    }
     cudaError_t e = cudaMemcpyFromSymbol(status, g_attn_status, sizeof(int));
     if (e == cudaSuccess && clear && *status != 0) {
         const int zero = 0;

@@ -31,6 +31,7 @@
 namespace b200q {
 
 __device__ int g_attn_prompt_status = 0;
+static std::atomic<bool> g_launched{false}; // nothing to read before
 
 constexpr int kPrThreads = 384;
 constexpr int kPrRows = 256; // rows of a unit
@@ -1011,6 +1012,7 @@ static_assert(kSMs * 2 <= kAttnCounters, "a counter for every CTA and tile");
 size_t attn_prompt_part_bytes(int head_dim) { return (size_t)kSMs * 4 * pr_part_floats(head_dim) * sizeof(float); }
 
 cudaError_t launch_attn_prompt(cudaStream_t s, AttnDev a) {
+    g_launched = true;
     a.min_tiles = 2;
     a.vec = !((uintptr_t)a.q & 15) && !((uintptr_t)a.out & 15) && !(a.q_stride & 3) && !(a.out_stride & 3);
     switch (a.kv.type) {
@@ -1021,6 +1023,10 @@ cudaError_t launch_attn_prompt(cudaStream_t s, AttnDev a) {
 }
 
 cudaError_t read_attn_prompt_status(int * status, bool clear) {
+    if (!g_launched) {
+        *status = 0;
+        return cudaSuccess;
+    }
     cudaError_t e = cudaMemcpyFromSymbol(status, g_attn_prompt_status, sizeof(int));
     if (e == cudaSuccess && clear && *status != 0) {
         const int zero = 0;

@@ -1,6 +1,8 @@
 // Paged KV cache and step batch as the kernels see them, and what they share: the rows of a sequence,
 // the keys they see, the page of a key, conversion to the cache's element types.
 #pragma once
+#include <atomic>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

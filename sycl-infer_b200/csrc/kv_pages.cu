@@ -5,6 +5,7 @@
 namespace b200q {
 
 __device__ int g_pages_status = 0;
+static std::atomic<bool> g_launched{false}; // nothing to read before
 
 constexpr int kCopyThreads = 256;
 
@@ -79,6 +80,7 @@ int kv_copy_chunks(const KvDev & c) { return (int)((page_value_bytes(c) + kCopyC
 
 cudaError_t launch_kv_copy_pages(cudaStream_t s, const KvDev & c, void * const * pools, int n_pools, const int32_t * src,
                                  const int32_t * dst, int n) {
+    g_launched = true;
     CopyArgs a = {};
     for (int i = 0; i < n_pools; i++) {
         a.pool[i] = static_cast<uint8_t *>(pools[i]);
@@ -110,6 +112,10 @@ cudaError_t launch_kv_remap(cudaStream_t s, const int32_t * table, int table_str
 }
 
 cudaError_t read_pages_status(int * status, bool clear) {
+    if (!g_launched) {
+        *status = 0;
+        return cudaSuccess;
+    }
     cudaError_t e = cudaMemcpyFromSymbol(status, g_pages_status, sizeof(int));
     if (e == cudaSuccess && clear && *status != 0) {
         const int zero = 0;

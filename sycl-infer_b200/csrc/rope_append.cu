@@ -18,6 +18,7 @@
 namespace b200q {
 
 __device__ int g_append_status = 0;
+static std::atomic<bool> g_launched{false}; // nothing to read before
 
 constexpr int kRopeThreads = 128;
 constexpr int kMaxRot = 128;
@@ -253,6 +254,7 @@ template <int T> static cudaError_t launch_append_t(cudaStream_t s, AppendArgs &
 cudaError_t launch_rope_append(cudaStream_t s, const double * table, int n_rot, int interleaved, const float * q,
                                int q_stride, int n_head, const float * k, int k_stride, const float * v, int v_stride,
                                float * q_out, int q_out_stride, const KvDev & kv, const BatchDev & b) {
+    g_launched = true;
     AppendArgs a = {};
     a.table = table;
     a.q = q;
@@ -294,6 +296,10 @@ cudaError_t launch_rope_table(cudaStream_t s, const b200q_rope & r, double * tab
 }
 
 cudaError_t read_append_status(int * status, bool clear) {
+    if (!g_launched) {
+        *status = 0;
+        return cudaSuccess;
+    }
     cudaError_t e = cudaMemcpyFromSymbol(status, g_append_status, sizeof(int));
     if (e == cudaSuccess && clear && *status != 0) {
         const int zero = 0;

@@ -304,3 +304,30 @@ def test_arguments_beyond_32_bits_are_refused(be, pkg):
     be.attn(q, out, cache, batch, scratch, window=2 ** 31 - 1, n_sink=2 ** 31 - 1, scale=1e-40)
     be.synchronize()
     assert torch.allclose(out[0].double(), dense[0][1][0].mean(0), atol=1e-5, rtol=0)  # no score counts
+
+
+@pytest.mark.gpu
+def test_status_of_kernels_that_have_run(pkg):
+    """In a process of its own: the status reads nothing of kernels that have not been launched, and each kernel's bad page
+    from its first launch on."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, __graft_entry__ as graft
+pkg = graft.load_package()
+be = pkg.make_cuda_backend(0)
+assert be.device_status() == 0
+i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+pool = torch.zeros(4, 1, 16, 64, dtype=torch.float16, device="cuda")
+cache, x, out = pkg.kv_cache(pool, pool.clone()), torch.zeros(20, 64, device="cuda"), torch.zeros(20, 64, device="cuda")
+one, many = (pkg.kv_batch(i32([[0, 9]]), i32([0, n]), i32([20]), n, n) for n in (1, 20))
+for call in (lambda: be.kv_copy_pages([cache], i32([0]), i32([7])), lambda: be.rope_append(None, None, x[:1], x[:1], None, cache, one),
+             lambda: be.attn(x[:1], out[:1], cache, one, pkg.alloc_attn_scratch(1, cache, one)),
+             lambda: be.attn(x, out, cache, many, pkg.alloc_attn_scratch(1, cache, many))):
+    call()
+    be.synchronize()
+    assert be.device_status() == 1 and be.device_status() == 0
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)
