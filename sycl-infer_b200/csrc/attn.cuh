@@ -18,7 +18,6 @@ struct AttnDev {
     int32_t window, n_sink;
     float * parts;       // scratch: what CTAs leave of units that they share
     uint32_t * counters; // scratch: arrivals at a unit that workers share, by the worker that has its start; zero between calls
-    int32_t min_tiles;   // prompts: tiles that a CTA gets at least
     int32_t vec;         // rows of q and out can be read and written 16 bytes at a time
 };
 

@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
     __shared__ int2 s_meta[WARPS][STAGES];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * kDecStageBytes;
-    float * join = reinterpret_cast<float *>(smem + WARPS * STAGES * kDecStageBytes); // TEAM 4: two parts
+    float * join = reinterpret_cast<float *>(smem + WARPS * STAGES * kDecStageBytes); // TEAM 8: four parts
 
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -208,8 +208,9 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
     } else {
         const long long units = total >> kUnitBit;
         total &= (1LL << kUnitBit) - 1;
-        // pieces of `each` tiles are at most total / each + units in number
-        each = units < gridDim.x ? (total + gridDim.x - units - 1) / (gridDim.x - units) : total;
+        // Pieces of `each` tiles are at most total / each + units in number: no more than CTAs, one for each at most (units
+        // are fewer than CTAs: kTeamUnits, one row block each).
+        each = (total + gridDim.x - units - 1) / (gridDim.x - units);
         each = each > TEAM ? each : TEAM; // a tile for every warp
         v_team = seq_workers(tid);
         sum_team = nw = block_sum(v_team, before_team);
@@ -223,10 +224,7 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
     auto share = [&](int w) { return w * each + (w < more ? w : more); };
     const int w_first = TEAM == 1 ? 0 : warp; // the warp's first tile of a segment
     const int copy_row = lane / CPR, copy_chunk = lane % CPR;
-    for (int worker = blockIdx.x * WORKERS + warp / TEAM;; worker += (int)gridDim.x * WORKERS) {
-    if (TEAM > 1 && worker >= nw) {
-        break;
-    }
+    const int worker = blockIdx.x * WORKERS + warp / TEAM;
     // ---- where the worker starts
     {
         long long run = 0;
@@ -804,11 +802,6 @@ __global__ void __launch_bounds__(dec_warps(TEAM) * 32, dec_per_sm(D, H8, TEAM))
         advance(sg, left, sq);
     }
     cp_async_wait<0>();
-    if constexpr (TEAM == 1) {
-        return;
-    }
-    __syncthreads(); // s_seq and the join space are used again
-    }
 }
 
 template <int T, int D, bool H8, int TEAM> static cudaError_t launch_t(cudaStream_t s, const AttnDev & a) {
@@ -830,9 +823,9 @@ template <int T, int D, bool H8, int TEAM> static cudaError_t launch_t(cudaStrea
     return cudaLaunchKernelEx(&cfg, attn_decode_kernel<T, D, H8, TEAM>, a);
 }
 
-// How a call is cut.  Few units: teams, so that a unit is left in few parts (B200, f16, 128 values, 8 KV heads: 2, 4, 8, 16
-// sequences of up to 8192 keys 30, 31, 46, 62 us with teams of four, 71, 41, 48, 61 us with warps alone).
-// (teams of eight: 14, 17, 31 us with 2, 4, 8; 33 against 47 with 9, 59 against 54 with 12.)
+// How a call is cut.  Few units: teams, so that a unit is left in few parts (B200, f16, 128 values, 8 KV heads, up to 8192
+// keys: 2, 4, 8 sequences 14, 17, 31 us with teams of eight, 71, 41, 48 us with warps alone; 9 sequences 33 against 47 us, 12
+// sequences 59 against 54: the border lies at half as many units as SMs).
 // Rows: as many as there are, up to eight or up to sixteen; e4m3 in many units takes eight in any case, since its
 // conversions and not its bytes bound it and many sequences have fewer rows than the largest (192 x window 1024 keys,
 // 4 to 12 rows: 88 -> 70 us; sixteen rows in all: 116 against 117 us).

@@ -160,6 +160,7 @@ struct PromptUnit {
 // A CTA's share of the list is measured in tiles plus kPrUnitCost a unit (its q, its join, its rows out): tile i of a unit
 // that starts at position `pos` of the list lies at pos + kPrUnitCost + i.
 constexpr int kPrUnitCost = 3;
+constexpr int kPrMinShare = 2; // smallest share in positions of the list (one that lies in a unit's fixed cost holds no tile)
 struct PromptSeg {
     int s, h, rb;
     int t_begin, t_end;
@@ -919,7 +920,7 @@ template <int T, int D> __global__ void __launch_bounds__(kPrThreads, 1) attn_pr
         int s, rb;
         total += block_scan(cost(p0 + tid, s, rb), before) * a.kv.n_kv;
     }
-    const long long want = (total + a.min_tiles - 1) / a.min_tiles;
+    const long long want = (total + kPrMinShare - 1) / kPrMinShare;
     const long long nw = max(1LL, want < gridDim.x ? want : gridDim.x);
     p.share.each = total / nw;
     p.share.more = total - p.share.each * nw;
@@ -965,10 +966,7 @@ template <int T, int D> __global__ void __launch_bounds__(kPrThreads, 1) attn_pr
         u = p.unit(seg.s, seg.rb);
         seg.t_begin = max(0, found[3] - kPrUnitCost);
         seg.t_end = (int)min((long long)u.k.count, p.share.end - seg.pos - kPrUnitCost);
-        work = seg.t_end > seg.t_begin; // a share may end inside a unit's fixed cost
-        if (!work && seg.pos + u.k.count + kPrUnitCost < p.share.end) {
-            work = p.advance(seg, u);
-        }
+        work = seg.t_end > seg.t_begin; // a share may end inside a unit's fixed cost, and has no tile then
     }
     if (work) {
         if (warp < 8) {
@@ -1013,7 +1011,6 @@ size_t attn_prompt_part_bytes(int head_dim) { return (size_t)kSMs * 4 * pr_part_
 
 cudaError_t launch_attn_prompt(cudaStream_t s, AttnDev a) {
     g_launched = true;
-    a.min_tiles = 2;
     a.vec = !((uintptr_t)a.q & 15) && !((uintptr_t)a.out & 15) && !(a.q_stride & 3) && !(a.out_stride & 3);
     switch (a.kv.type) {
     case kF16: return a.kv.head_dim == 64 ? launch_t<kF16, 64>(s, a) : launch_t<kF16, 128>(s, a);
