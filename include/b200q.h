@@ -312,8 +312,10 @@ int b200q_i8_block_dots(void * stream, const void * w, uint32_t type, int K, int
                         int t, int32_t * wd);
 
 /* Device-side error word.  Kernels never spin without a limit: a wait that runs out stores
- * B200Q_ETIMEOUT here and the kernel returns.  Synchronizes with the device (reads a device
- * symbol); `clear` != 0 resets the word after reading.  No counterpart in the reference,
+ * B200Q_ETIMEOUT here and the kernel returns.  A page id outside the pool (attention side) stores
+ * B200Q_EINVAL, which a wait that ran out takes precedence over: after the one a key is left out, after the
+ * other the results are lost.  Synchronizes with the device (reads device
+ * symbols); `clear` != 0 resets the words after reading.  No counterpart in the reference,
  * whose kernels have no device-side waits. */
 int b200q_device_status(int * status /*host*/, int clear);
 
@@ -397,7 +399,7 @@ int b200q_rope_table(void * stream, const b200q_rope * rope /*host*/, double * t
  * cache.  q, k, v: fp32 rows of n_head * head_dim, n_kv * head_dim values, as the q|k|v call leaves them
  * (views of one buffer included).  table NULL: no rotation.  q NULL: only the append; k and v NULL (both): only
  * the rotation of q.  Angles are formed in 64 bits, so far positions keep fp32 accuracy.  Values
- * beyond the range of an F16 or E4M3 cache are stored as its largest finite value; NaN stays NaN. */
+ * beyond the range of the cache's type, infinities among them, are stored as its largest finite value; NaN stays NaN. */
 int b200q_rope_append(void * stream, const double * table, const b200q_rope * rope /*host*/, const float * q,
                       int q_stride, int n_head, const float * k, int k_stride, const float * v, int v_stride,
                       float * q_out, int q_out_stride, const b200q_kv_cache * cache /*host*/,

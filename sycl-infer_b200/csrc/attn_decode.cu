@@ -27,7 +27,7 @@
 // * Join.  Where a unit spans workers, each leaves its (m, l, o) in the scratch and the one that finishes last joins the
 //   parts in order, so results do not depend on who that is.
 //
-// B200: 1 x 131071 keys bf16 (537 MB) 96 us, of which the stream takes 72 (7.5 TB/s), the start 4, the spread of the
+// B200: 1 x 131071 keys bf16 (537 MB) 93 us, of which the stream takes 72 (7.5 TB/s), the start 4, the spread of the
 // CTAs' ends and the last join the rest; 32 x 200..8192 keys f16 (595 MB) 107 us, 5.5 TB/s: the shares are equal, the SMs' rates
 // are not (ends from 70 to 99 us); 192 x window 1024 e4m3 62 us: widening 8-bit keys in registers is what it issues.
 #include "async.cuh"

@@ -22,8 +22,10 @@
 // B200: 512 tokens after 32001 keys f16 591 us alone, 710 us in a run of them at the power limit: 1.14 and 0.95 PFLOP/s of tensor
 // work (the two parts), 69 % of the measured burst and 69 % of the sustained bf16 rate.  A step of two tiles takes
 // 7600 clocks of which the tensor pipe works 54 %; the softmax of a tile takes 4500, two thirds of it loads from tensor memory
-// that nothing hides (330 clocks each while products run).  Wider loads (64 columns) spill and lose: 672 us.  Prompts of 2048
-// tokens bf16 (122 us) and short windows are bound by what a unit costs beside its tiles: q in, rows out, the first scores (about 9 us).
+// that nothing hides (330 clocks each while products run).  Wider loads (64 columns) spill and lose: 672 us.  The same step is most of
+// the other prompts: 2048 tokens bf16 125 us, of which a CTA's 18.6 steps of two tiles take 74 and what its 2.8 units cost beside
+// them (q in, first scores, rows out: about 9 us each, one after the other) 25; window 512 over 64 values, e4m3, 142 us: 24 steps
+// and 4.5 units, some 90 and 40.
 // bf16 keys widened to fp16 by the producers, for 22 bits there too, made the prompt of 2048 tokens 270 us: not taken.
 #include "async.cuh"
 #include "attn.cuh"
