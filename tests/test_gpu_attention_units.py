@@ -331,3 +331,70 @@ for call in (lambda: be.kv_copy_pages([cache], i32([0]), i32([7])), lambda: be.r
 """
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("typ", ["bf16", "e4m3"])
+def test_a_recorded_step_of_every_call(be, pkg, typ):
+    """Append, prompt and decode attention on one scratch, page copies and the remap, recorded into two graphs that share the
+    scratch and run in turn: with other lengths, rows, tables and page lists each time, the bits of the calls one by one."""
+    n_kv, group, dim, page, n_tok, n_seq = 2, 5, 64, 16, 160, 3
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    rope = pkg.rope_t(dim, base=1e4)
+    be.rope_table(rope)
+    qd, kd = n_kv * group * dim, n_kv * dim
+
+    def state():
+        gen = torch.Generator().manual_seed(3)
+        pools = [torch.randn(64, n_kv, page, dim, generator=gen).to(TYPES[typ]).cuda() for _ in range(2)]
+        d = dict(pools=pools, table=torch.zeros(n_seq, 20, dtype=torch.int32, device="cuda"), first=i32([0] * (n_seq + 1)),
+                 len=i32([0] * n_seq), one=i32([0, 1, 2, 3]), qkv=torch.zeros(n_tok, qd + 2 * kd, device="cuda"), src=i32([0, 1]),
+                 dst=i32([2, 3]), map=torch.arange(64, dtype=torch.int32, device="cuda"), mapped=torch.zeros(n_seq, 20, dtype=torch.int32, device="cuda"),
+                 out=torch.zeros(n_tok, qd, device="cuda"), last=torch.zeros(n_seq, qd, device="cuda"), q1=torch.zeros(n_seq, qd, device="cuda"))
+        d["cache"] = pkg.kv_cache(*pools)
+        d["batch"] = pkg.kv_batch(d["table"], d["first"], d["len"], n_tok, n_tok)
+        d["step"] = pkg.kv_batch(d["table"], d["one"], d["len"], n_seq, 1)
+        return d
+
+    def run(d, scratch):
+        q, k, v = d["qkv"].split([qd, kd, kd], 1)
+        be.kv_copy_pages([d["cache"]], d["src"], d["dst"])
+        be.rope_append(rope, q, k, v, q, d["cache"], d["batch"])
+        be.attn(q, d["out"], d["cache"], d["batch"], scratch, window=70, n_sink=3)
+        be.attn(d["q1"], d["last"], d["cache"], d["step"], scratch)
+        be.kv_remap(d["table"], d["map"], d["mapped"])
+
+    plain, recorded, again = state(), state(), state()
+    scratch = torch.zeros(max(pkg.alloc_attn_scratch(n_kv * group, plain["cache"], plain[b]).nbytes for b in ("batch", "step")), dtype=torch.uint8, device="cuda")
+    stream, graphs = torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    for d in (recorded, again):
+        with torch.cuda.stream(stream):
+            run(d, scratch)  # no rows, no keys
+            stream.synchronize()
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=stream):
+                run(d, scratch)
+    run(plain, scratch)  # from here on the three pools are the same: pages 2 and 3 hold what 0 and 1 do
+    gen = torch.Generator().manual_seed(4)
+    for rows, lens in (([100, 1, 59], [200, 1, 300]), ([0, 160, 0], [16, 160, 0]), ([1, 1, 1], [317, 18, 31]), ([40, 0, 33], [40, 250, 20])):
+        pages = torch.randperm(64, generator=gen).to(torch.int32)
+        new = dict(table=pages[:60].view(3, 20), len=torch.tensor(lens, dtype=torch.int32), src=pages[60:62], dst=pages[62:64],
+                   first=torch.tensor([0, *rows], dtype=torch.int32).cumsum(0, dtype=torch.int32), map=torch.randperm(64, generator=gen).to(torch.int32),
+                   qkv=torch.randn(n_tok, qd + 2 * kd, generator=gen), q1=torch.randn(n_seq, qd, generator=gen))
+        for d in (plain, recorded, again):
+            for name, x in new.items():
+                d[name].copy_(x)
+            d["out"].fill_(7.0)
+        torch.cuda.synchronize()
+        run(plain, scratch)
+        torch.cuda.synchronize()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for d in (recorded, again):
+            for name in ("out", "last", "mapped", "qkv"):
+                assert torch.equal(d[name], plain[name]), name
+            assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(d["pools"], plain["pools"]))
+        assert bool((plain["out"][sum(rows):] == 7).all()) and float(plain["last"].abs().max()) > 0
+        assert be.device_status() == 0
