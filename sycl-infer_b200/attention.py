@@ -8,6 +8,7 @@ in src/engine/engine_prefix_cache).
 """
 import ctypes as C
 import heapq
+import operator
 from dataclasses import dataclass, field
 
 import torch
@@ -26,7 +27,7 @@ def _int(value, what):
     """An int32 of the C structs, of which ctypes would silently keep the low bits; what is too small the library refuses."""
     if not -2 ** 31 <= value < 2 ** 31:
         raise ValueError(f"{what}: {value} does not fit 32 bits")
-    return int(value)
+    return operator.index(value)  # no fractions
 
 
 class kv_cache:
@@ -71,7 +72,7 @@ class kv_batch:
             raise ValueError("kv_batch: page_table must be contiguous")
         self.page_table, self.q_start, self.kv_len = page_table, q_start, kv_len
         self.device, self.n_seq = kv_len.device, n_seq
-        self.n_tok, self.max_q = _int(n_tok, "kv_batch: n_tok"), _int(max_q, "kv_batch: max_q")
+        self.n_tok, self.max_q = _int(int(n_tok), "kv_batch: n_tok"), _int(int(max_q), "kv_batch: max_q")
         self.c = KvBatch(page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), stride, n_seq, self.n_tok, self.max_q)
         self.ref = C.byref(self.c)
 

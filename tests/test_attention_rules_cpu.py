@@ -118,6 +118,9 @@ def test_counts_beyond_32_bits_are_refused(pkg):
         with pytest.raises(ValueError):
             pkg.rope_t(**kw)
 
+    with pytest.raises(TypeError):
+        pkg.rope_t(64.5)
+
     class view:  # rows that far apart take more memory than there is
         dtype, shape = torch.float32, (2, 256)
         get_device, data_ptr = (lambda self: 0), (lambda self: 1 << 20)
